@@ -14,6 +14,7 @@ CSRC_DIR = os.path.join(_HERE, "csrc")
 _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
 _c_i64 = ctypes.c_int64
+_c_float = ctypes.c_float
 _i32_p = ctypes.POINTER(ctypes.c_int32)
 
 # name -> (restype, argtypes); must list every symbol include/moe_gg.h declares.
@@ -80,6 +81,26 @@ SIGNATURES = {
     "moe_gg_fp8_groupwise_quant": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_i64, _c_void_p]),
     "moe_gg_fp8_block128_quant": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_i64, _c_int, _c_void_p]),
     "moe_gg_align_block_size": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "moe_gg_route_gate": (_c_int, [_c_void_p, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p, _c_void_p, _c_void_p]),
+    "moe_gg_route_gate_backward": (
+        _c_int, [_c_void_p, _c_void_p, _c_int, _c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p, _c_void_p]),
+    "moe_gg_block_norm": (
+        _c_int, [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_float, _c_float, _c_float, _c_void_p,
+                 _c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_void_p]),
+    "moe_gg_block_norm_backward_workspace": (ctypes.c_size_t, [_c_i64, _c_int]),
+    "moe_gg_block_norm_backward": (
+        _c_int, [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_float,
+                 _c_float, _c_float, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_void_p,
+                 ctypes.c_size_t, _c_void_p]),
+    "moe_gg_lora_plan": (_c_int, [_c_void_p, _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "moe_gg_lora_add_workspace": (ctypes.c_size_t, [_c_i64, _c_int, _c_int, _c_int, _c_int]),
+    "moe_gg_lora_add": (
+        _c_int, [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_i64, _c_int, _c_int,
+                 _c_int, _c_void_p, _c_i64, _c_void_p, _c_int, _c_void_p, ctypes.c_size_t, _c_void_p]),
+    "moe_gg_lora_backward_workspace": (ctypes.c_size_t, [_c_i64, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "moe_gg_lora_backward": (
+        _c_int, [_c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_i64, _c_int, _c_int,
+                 _c_int, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_int, _c_void_p, ctypes.c_size_t, _c_void_p]),
     "moe_gg_host_enumerate_tiles": (
         _c_int,
         [_i32_p, _c_int, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _i32_p, _c_int],

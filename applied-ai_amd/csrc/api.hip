@@ -73,6 +73,33 @@ bool use_streaming_kernel(int64_t M, int G, int64_t ntn256, int num_wg) {
 // 2048-14336); with four fragments it falls behind them.
 bool use_decode_kernel(int64_t M, int G) { return M <= (int64_t)G * 24; }
 
+// Shared argument checks of the gate, the norms and the adapters.
+int check_gate(const void* logits, int dtype, int64_t T, int E, int k, int score) {
+  if (dtype != MOE_GG_DTYPE_FP32 && dtype != MOE_GG_DTYPE_BF16 && dtype != MOE_GG_DTYPE_FP16) return MOE_GG_EINVAL;
+  if (score != MOE_GG_GATE_SOFTMAX && score != MOE_GG_GATE_SIGMOID) return MOE_GG_EINVAL;
+  if (k > E) return MOE_GG_ESHAPE;
+  if (E > MOE_GG_MAX_ROUTE_EXPERTS || k > 64 || T > (1 << 24)) return MOE_GG_EUNSUPPORTED;
+  if (T == 0 || E == 0) return MOE_GG_OK;
+  if (!logits) return MOE_GG_EINVAL;
+  return aligned(logits, dtype == MOE_GG_DTYPE_FP32 ? 4 : 2) ? MOE_GG_OK : MOE_GG_EALIGN;
+}
+
+int check_norm(int64_t T, int d, int gate_kind, int dtype, int stream_dtype, int weight_dtype) {
+  if (T < 0 || d < 0 || gate_kind < MOE_GG_GATE_NONE || gate_kind > MOE_GG_GATE_ROW) return MOE_GG_EINVAL;
+  if (dtype != MOE_GG_DTYPE_BF16 && dtype != MOE_GG_DTYPE_FP16) return MOE_GG_EINVAL;
+  if (stream_dtype != dtype && stream_dtype != MOE_GG_DTYPE_FP32) return MOE_GG_EINVAL;
+  if (weight_dtype != dtype && weight_dtype != MOE_GG_DTYPE_FP32) return MOE_GG_EINVAL;
+  return d > MOE_GG_MAX_NORM_WIDTH || T > (1 << 21) ? MOE_GG_EUNSUPPORTED : MOE_GG_OK;
+}
+
+int check_lora_sizes(int L, int64_t T, int K, int N, int R) {
+  if (L < 0 || T < 0 || K < 0 || N < 0 || R < 0) return MOE_GG_EINVAL;
+  if (K == 0 || N == 0 || R == 0) return MOE_GG_ESHAPE;
+  // a grid holds fewer than 2^32 threads: slots of rows times column blocks stay below that
+  if (R > MOE_GG_MAX_LORA_RANK || L > MOE_GG_MAX_LORA_ADAPTERS || K > (1 << 17) || N > (1 << 17) || T > (1 << 20)) return MOE_GG_EUNSUPPORTED;
+  return MOE_GG_OK;
+}
+
 }  // namespace
 
 // The ping-pong kernels form slab offsets with 24-bit multiplies: an operand row must be shorter than 16 MB.
@@ -763,6 +790,144 @@ int moe_gg_host_enumerate_tiles_two_lists(const int32_t* m_sizes_host, int G, in
     }
   }
   return written;
+}
+
+int moe_gg_route_gate(const void* logits, int dtype, int64_t T, int E, int k, int score, int renormalize, float scale,
+                      float* weights, int32_t* ids, void* stream) {
+  if (T < 0 || E < 0 || k < 0) return MOE_GG_EINVAL;
+  const int rc = check_gate(logits, dtype, T, E, k, score);
+  if (rc != MOE_GG_OK || T == 0 || k == 0) return rc;
+  if (!weights || !ids) return MOE_GG_EINVAL;
+  if (!aligned(weights, 4) || !aligned(ids, 4)) return MOE_GG_EALIGN;
+  GateParams p{logits, dtype, (int)T, E, k, scale, weights, ids, nullptr};
+  return (int)gate_launch(p, score == MOE_GG_GATE_SIGMOID, renormalize != 0, (hipStream_t)stream);
+}
+
+int moe_gg_route_gate_backward(const float* grad_weights, const void* logits, int dtype, const int32_t* ids, int64_t T, int E, int k,
+                               int score, int renormalize, float scale, void* grad_logits, void* stream) {
+  if (T < 0 || E < 0 || k < 0) return MOE_GG_EINVAL;
+  const int rc = check_gate(logits, dtype, T, E, k, score);
+  if (rc != MOE_GG_OK || T == 0 || E == 0) return rc;
+  if (!grad_logits || (k > 0 && (!grad_weights || !ids))) return MOE_GG_EINVAL;
+  if (!aligned(grad_weights, 4) || !aligned(ids, 4) || !aligned(grad_logits, dtype == MOE_GG_DTYPE_FP32 ? 4 : 2)) return MOE_GG_EALIGN;
+  GateParams p{logits, dtype, (int)T, E, k, scale, const_cast<float*>(grad_weights), const_cast<int32_t*>(ids), grad_logits};
+  return (int)gate_launch(p, score == MOE_GG_GATE_SIGMOID, renormalize != 0, (hipStream_t)stream);
+}
+
+int moe_gg_block_norm(const void* y, int64_t ldy, const void* residual, int64_t ldr, const void* w_post, const void* gate,
+                      int gate_kind, const void* w_pre, float residual_scale, float block_scale, float eps, void* h, void* z,
+                      int64_t T, int d, int dtype, int stream_dtype, int weight_dtype, void* stream) {
+  const int rc = check_norm(T, d, gate_kind, dtype, stream_dtype, weight_dtype);
+  if (rc != MOE_GG_OK) return rc;
+  if (T == 0 || d == 0) return MOE_GG_OK;
+  if (!residual || (y && !h) || (w_pre && !z) || (!y && !w_pre) || (gate_kind != MOE_GG_GATE_NONE) != (gate != nullptr)) return MOE_GG_EINVAL;
+  if (!y && (w_post || gate || h || residual_scale != 1.f)) return MOE_GG_EINVAL;
+  if ((y && ldy < d) || ldr < d) return MOE_GG_ESHAPE;
+  const size_t es = stream_dtype == MOE_GG_DTYPE_FP32 ? 4 : 2, ew = weight_dtype == MOE_GG_DTYPE_FP32 ? 4 : 2;
+  if (!aligned(y, 2) || !aligned(z, 2) || !aligned(residual, es) || !aligned(h, es) || !aligned(w_post, ew) || !aligned(w_pre, ew) || !aligned(gate, ew))
+    return MOE_GG_EALIGN;
+  NormParams p{};
+  p.y = y; p.res = residual; p.ldy = y ? ldy : 0; p.ldr = ldr; p.w_post = w_post; p.gate = gate; p.gate_kind = gate_kind; p.w_pre = w_pre;
+  p.alpha = residual_scale; p.beta = block_scale; p.eps = eps; p.h = h; p.z = z; p.T = (int)T; p.d = d;
+  p.wide = stream_dtype == MOE_GG_DTYPE_FP32; p.wide_w = weight_dtype == MOE_GG_DTYPE_FP32;
+  return (int)block_norm_launch(p, dtype == MOE_GG_DTYPE_FP16, (hipStream_t)stream);
+}
+
+size_t moe_gg_block_norm_backward_workspace(int64_t T, int d) {
+  return T > 0 && d > 0 && d <= MOE_GG_MAX_NORM_WIDTH ? block_norm_backward_workspace(T, d) : 0;
+}
+
+int moe_gg_block_norm_backward(const void* grad_h, int64_t ldgh, const void* grad_z, int64_t ldgz, const void* y, int64_t ldy, const void* h,
+                               int64_t ldh, const void* w_post, const void* gate, int gate_kind, const void* w_pre,
+                               float residual_scale, float block_scale, float eps, void* grad_y, void* grad_residual, void* grad_w_post,
+                               void* grad_gate, void* grad_w_pre, int64_t T, int d, int dtype, int stream_dtype, int weight_dtype,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_norm(T, d, gate_kind, dtype, stream_dtype, weight_dtype);
+  if (rc != MOE_GG_OK) return rc;
+  if (d == 0) return MOE_GG_OK;
+  if ((y != nullptr) != (grad_y != nullptr) || (w_pre != nullptr) != (grad_z != nullptr) || !grad_residual || (w_pre && !h)) {
+    if (T != 0) return MOE_GG_EINVAL;
+  }
+  if ((w_post != nullptr) != (grad_w_post != nullptr) || (w_pre != nullptr) != (grad_w_pre != nullptr) ||
+      (gate_kind != MOE_GG_GATE_NONE) != (gate != nullptr) || (gate != nullptr) != (grad_gate != nullptr))
+    return MOE_GG_EINVAL;
+  if (!y && T != 0 && (w_post || gate || residual_scale != 1.f)) return MOE_GG_EINVAL;
+  if (T != 0 && ((y && ldy < d) || (grad_h && ldgh < d) || (w_pre && (ldh < d || ldgz < d)))) return MOE_GG_ESHAPE;
+  const size_t es = stream_dtype == MOE_GG_DTYPE_FP32 ? 4 : 2, ew = weight_dtype == MOE_GG_DTYPE_FP32 ? 4 : 2;
+  if (!aligned(y, 2) || !aligned(grad_z, 2) || !aligned(grad_y, 2) || !aligned(h, es) || !aligned(grad_h, es) || !aligned(grad_residual, es) ||
+      !aligned(w_post, ew) || !aligned(w_pre, ew) || !aligned(gate, ew) || !aligned(grad_w_post, ew) || !aligned(grad_w_pre, ew) || !aligned(grad_gate, ew))
+    return MOE_GG_EALIGN;
+  if (T != 0) {
+    if (!workspace || workspace_bytes < block_norm_backward_workspace(T, d)) return MOE_GG_EINVAL;
+    if (!aligned(workspace, 256)) return MOE_GG_EALIGN;
+  }
+  NormGradParams p{};
+  p.gh = grad_h; p.gz = grad_z; p.y = y; p.h = h;
+  p.ldgh = grad_h ? ldgh : 0; p.ldgz = w_pre ? ldgz : 0; p.ldy = y ? ldy : 0; p.ldh = w_pre ? ldh : 0;
+  p.w_post = w_post; p.gate = gate; p.gate_kind = gate_kind; p.w_pre = w_pre; p.alpha = residual_scale; p.beta = block_scale; p.eps = eps;
+  p.gy = grad_y; p.gres = grad_residual; p.g_post = grad_w_post; p.g_gate = grad_gate; p.g_pre = grad_w_pre;
+  p.sums = (float*)workspace; p.T = (int)T; p.d = d; p.wide = stream_dtype == MOE_GG_DTYPE_FP32; p.wide_w = weight_dtype == MOE_GG_DTYPE_FP32;
+  return (int)block_norm_backward_launch(p, dtype == MOE_GG_DTYPE_FP16, (hipStream_t)stream);
+}
+
+int moe_gg_lora_plan(const int32_t* ids, int64_t T, int L, int32_t* perm, int32_t* offsets, int32_t* scratch, void* stream) {
+  if (T < 0 || L < 0) return MOE_GG_EINVAL;
+  if (T > INT32_MAX || L > MOE_GG_MAX_LORA_ADAPTERS) return MOE_GG_EUNSUPPORTED;
+  if (!offsets || !scratch || (T > 0 && (!ids || !perm))) return MOE_GG_EINVAL;
+  if (!aligned(ids, 4) || !aligned(perm, 4) || !aligned(offsets, 4) || !aligned(scratch, 4)) return MOE_GG_EALIGN;
+  return (int)lora_plan_launch(ids, (int)T, L, perm, offsets, scratch, (hipStream_t)stream);
+}
+
+size_t moe_gg_lora_add_workspace(int64_t T, int L, int K, int N, int R) {
+  return check_lora_sizes(L, T, K, N, R) == MOE_GG_OK && T > 0 ? lora_forward_workspace(T, L, K, N, R) : 0;
+}
+
+size_t moe_gg_lora_backward_workspace(int64_t T, int L, int K, int N, int R, int with_h) {
+  return check_lora_sizes(L, T, K, N, R) == MOE_GG_OK ? lora_backward_workspace(T, L, K, N, R, with_h != 0) : 0;
+}
+
+int moe_gg_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, const void* a, const void* b, const float* scales,
+                    const int32_t* perm, const int32_t* offsets, int L, int64_t T, int K, int N, int R, void* out, int64_t ldo,
+                    float* h, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_lora_sizes(L, T, K, N, R);
+  if (rc != MOE_GG_OK) return rc;
+  if (dtype != MOE_GG_DTYPE_BF16 && dtype != MOE_GG_DTYPE_FP16) return MOE_GG_EINVAL;
+  if (T == 0) return MOE_GG_OK;
+  if (ldy < N || ldo < N || ldx < K || (out == y && ldo != ldy)) return MOE_GG_ESHAPE;
+  if (!y || !x || !out || !perm || !offsets || (L > 0 && (!a || !b)) || !workspace) return MOE_GG_EINVAL;
+  if (!aligned(y, 2) || !aligned(x, 2) || !aligned(out, 2) || !aligned(a, 2) || !aligned(b, 2) || !aligned(scales, 4) || !aligned(h, 4) ||
+      !aligned(perm, 4) || !aligned(offsets, 4) || !aligned(workspace, 256))
+    return MOE_GG_EALIGN;
+  if (workspace_bytes < lora_forward_workspace(T, L, K, N, R)) return MOE_GG_EINVAL;
+  LoraParams p{};
+  p.y = y; p.ldy = ldy; p.x = x; p.ldx = ldx; p.a = a; p.b = b; p.scales = scales; p.perm = perm; p.offsets = offsets;
+  p.L = L; p.T = (int)T; p.K = K; p.N = N; p.R = R; p.out = out; p.ldo = ldo; p.h = h; p.workspace = workspace;
+  return (int)lora_forward_launch(p, dtype == MOE_GG_DTYPE_FP16, (hipStream_t)stream);
+}
+
+int moe_gg_lora_backward(const void* grad_out, int64_t ldg, const void* x, int64_t ldx, const void* a, const void* b, const float* scales,
+                         const int32_t* perm, const int32_t* offsets, int L, int64_t T, int K, int N, int R, const float* h,
+                         const void* grad_x_in, int64_t ld_in, void* grad_x, int64_t ld_grad_x, void* grad_a, void* grad_b, int dtype,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+  const int rc = check_lora_sizes(L, T, K, N, R);
+  if (rc != MOE_GG_OK) return rc;
+  if (dtype != MOE_GG_DTYPE_BF16 && dtype != MOE_GG_DTYPE_FP16) return MOE_GG_EINVAL;
+  if (T > 0) {
+    if (ldg < N || ldx < K || ld_grad_x < K || (grad_x_in && ld_in < K) || (grad_x == grad_x_in && ld_grad_x != ld_in)) return MOE_GG_ESHAPE;
+    if (!grad_out || !x || !grad_x || !perm || !workspace) return MOE_GG_EINVAL;
+  } else if (L == 0) {
+    return MOE_GG_OK;
+  }
+  if (!offsets || (L > 0 && (!a || !b || !grad_a || !grad_b)) || !workspace) return MOE_GG_EINVAL;
+  if (!aligned(grad_out, 2) || !aligned(x, 2) || !aligned(grad_x, 2) || !aligned(grad_x_in, 2) || !aligned(a, 2) || !aligned(b, 2) || !aligned(grad_a, 2) ||
+      !aligned(grad_b, 2) || !aligned(scales, 4) || !aligned(h, 4) || !aligned(perm, 4) || !aligned(offsets, 4) || !aligned(workspace, 256))
+    return MOE_GG_EALIGN;
+  if (workspace_bytes < lora_backward_workspace(T, L, K, N, R, h != nullptr)) return MOE_GG_EINVAL;
+  LoraParams p{};
+  p.y = grad_out; p.ldy = ldg; p.x = x; p.ldx = ldx; p.a = a; p.b = b; p.scales = scales; p.perm = perm; p.offsets = offsets;
+  p.L = L; p.T = (int)T; p.K = K; p.N = N; p.R = R; p.h = const_cast<float*>(h); p.gx_in = grad_x_in; p.ld_gx_in = ld_in; p.gx = grad_x;
+  p.ld_gx = ld_grad_x; p.grad_a = grad_a; p.grad_b = grad_b; p.workspace = workspace;
+  return (int)lora_backward_launch(p, dtype == MOE_GG_DTYPE_FP16, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -138,3 +138,85 @@ hipError_t gg_bf16_pingpong_wgrad_launch(const GgParams& p, int num_wg, hipStrea
 // dW = dY^T X per expert on the transposed, padded operands; p.x = dY^T [N, ldm], p.w = X^T [K, ldm], p.M = ldm,
 // p.skip_rows = number of gradient rows (bound for m_sizes), p.y = dW [G * N, K] with p.ldy = K. block in {256, 128}.
 hipError_t gg_bf16_wgrad_launch(const GgParams& p, int block, int num_wg, hipStream_t stream);
+
+// Low-rank adapters (lora.hip). perm / offsets as lora_plan_launch writes them ([T] and [L + 2]); all matrices 16-bit floats of
+// one type, row-major. R <= MOE_GG_MAX_LORA_RANK.
+struct LoraParams {
+  const void* y;  // forward: [T, N] to add to; backward: the gradient of the output
+  int64_t ldy;
+  const void* x;  // [T, K]
+  int64_t ldx;
+  const void* a;  // [L, R, K]
+  const void* b;  // [L, N, R]
+  const float* scales;  // [L] or null: 1
+  const int32_t* perm;
+  const int32_t* offsets;
+  int L, T, K, N, R;
+  void* out;  // forward; may be y
+  int64_t ldo;
+  void* h;    // [T, R] fp32 or null: written by the forward pass, read by the backward pass
+  const void* gx_in;  // backward: [T, K] or null, may be gx
+  int64_t ld_gx_in;
+  void* gx;
+  int64_t ld_gx;
+  void* grad_a;
+  void* grad_b;
+  void* workspace;
+};
+size_t lora_forward_workspace(int64_t T, int L, int K, int N, int R);
+size_t lora_backward_workspace(int64_t T, int L, int K, int N, int R, bool with_h);
+// scratch: T + L + 1 int32
+hipError_t lora_plan_launch(const int32_t* ids, int T, int L, int32_t* perm, int32_t* offsets, int32_t* scratch, hipStream_t stream);
+hipError_t lora_forward_launch(const LoraParams& p, bool fp16, hipStream_t stream);
+hipError_t lora_backward_launch(const LoraParams& p, bool fp16, hipStream_t stream);
+
+// Router gate (gate.hip). logits [T, E] of dtype MOE_GG_DTYPE_*; E <= 768, k <= min(E, 64).
+struct GateParams {
+  const void* logits;
+  int dtype, T, E, k;
+  float scale;
+  float* weights;  // forward: out [T, k]; backward: their gradient
+  int32_t* ids;    // forward: out [T, k]; backward: in
+  void* grad_logits;  // backward only: out [T, E]
+};
+hipError_t gate_launch(const GateParams& p, bool sigmoid, bool renormalize, hipStream_t stream);
+
+// Norms before and after a block (block_norm.hip). T rows of d <= MOE_GG_MAX_NORM_WIDTH; y, z and their gradients 16 bits, the
+// stream (res, h, gres, gh) that type or, with wide, fp32; weights and gate that type or, with wide_w, fp32.
+struct NormParams {
+  const void* y;    // null: z is the norm of res
+  const void* res;
+  int64_t ldy, ldr;
+  const void* w_post;  // or null
+  const void* gate;
+  int gate_kind;       // 0: none, 1: [d], 2: [T]
+  const void* w_pre;   // or null: no z
+  float alpha, beta, eps;
+  void* h;
+  void* z;
+  int T, d;
+  bool wide, wide_w;
+};
+struct NormGradParams {
+  const void* gh;   // or null: zeros
+  const void* gz;   // with w_pre
+  const void* y;
+  const void* h;
+  int64_t ldgh, ldgz, ldy, ldh;
+  const void* w_post;
+  const void* gate;
+  int gate_kind;
+  const void* w_pre;
+  float alpha, beta, eps;
+  void* gy;
+  void* gres;
+  void* g_post;
+  void* g_gate;
+  void* g_pre;
+  float* sums;
+  int T, d, parts;
+  bool wide, wide_w;
+};
+size_t block_norm_backward_workspace(int64_t T, int d);
+hipError_t block_norm_launch(const NormParams& p, bool fp16, hipStream_t stream);
+hipError_t block_norm_backward_launch(NormGradParams p, bool fp16, hipStream_t stream);

@@ -92,3 +92,58 @@ def gather_sorted(x: torch.Tensor, perm: torch.Tensor, k: int, offsets: torch.Te
                                            offsets[-1:].data_ptr() if offsets is not None else None, _stream_ptr(dev))
     _lib.check(rc, "moe_gg_gather_rows")
     return out
+
+
+_SCORES = {"softmax": 0, "sigmoid": 1}                             # MOE_GG_GATE_SOFTMAX / _SIGMOID
+_LOGITS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # MOE_GG_DTYPE_*
+
+
+def _check_gate(logits: torch.Tensor, k: int, score: str) -> None:
+    if logits.dim() != 2 or logits.dtype not in _LOGITS:
+        raise ValueError("logits must be fp32, bf16 or fp16 [T, E]")
+    if score not in _SCORES:
+        raise ValueError("score must be 'softmax' or 'sigmoid'")
+    if not 1 <= k <= logits.shape[1]:
+        raise ValueError(f"k must be between 1 and the {logits.shape[1]} experts")
+
+
+def route_gate(logits: torch.Tensor, k: int, score: str = "softmax", renormalize: bool = True,
+               scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The router's gate: logits [T, E] -> (weights [T, k] fp32, ids [T, k] int32), the topk_weights and topk_ids of fused_moe.
+
+    ids are the k largest logits of a row in descending order, ties to the lower id (as route_topk); weights their softmax or
+    sigmoid scores, divided by their sum if renormalize, times scale. Switch an expert off by a logit of -inf: if it is chosen for
+    want of others its weight is 0, and a row of nothing else has weights of 0. fp32 arithmetic. k <= 64."""
+    _check_gate(logits, k, score)
+    dev = _require_cuda(logits)
+    logits = logits.contiguous()
+    T, E = logits.shape
+    weights = torch.empty((T, k), dtype=torch.float32, device=dev)
+    ids = torch.empty((T, k), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        rc = _lib.lib().moe_gg_route_gate(logits.data_ptr(), _LOGITS[logits.dtype], T, E, k, _SCORES[score], 1 if renormalize else 0, scale,
+                                          weights.data_ptr(), ids.data_ptr(), _stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "moe_gg_route_gate")
+    return weights, ids
+
+
+def route_gate_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, score: str = "softmax",
+                        renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """Gradient of route_gate's weights with respect to the logits, [T, E] in their type: grad_weights [T, k] fp32, logits and
+    ids [T, k] as route_gate took and returned them. The choice itself has no gradient; an id outside [0, E) takes no part."""
+    if ids.dim() != 2 or ids.dtype != torch.int32 or grad_weights.shape != ids.shape or grad_weights.dtype != torch.float32:
+        raise ValueError("ids must be int32 [T, k] and grad_weights fp32 of the same shape")
+    _check_gate(logits, ids.shape[1], score)
+    if ids.shape[0] != logits.shape[0]:
+        raise ValueError("ids and logits must have the same number of rows")
+    dev = _require_cuda(grad_weights, logits, ids)
+    grad_weights, logits, ids = grad_weights.contiguous(), logits.contiguous(), ids.contiguous()
+    T, E = logits.shape
+    grad = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    with torch.cuda.device(dev):
+        rc = _lib.lib().moe_gg_route_gate_backward(grad_weights.data_ptr(), logits.data_ptr(), _LOGITS[logits.dtype], ids.data_ptr(), T, E, ids.shape[1],
+                                                   _SCORES[score], 1 if renormalize else 0, scale, grad.data_ptr(), _stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "moe_gg_route_gate_backward")
+    return grad

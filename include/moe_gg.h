@@ -294,6 +294,89 @@ int moe_gg_fp8_groupwise_quant(const void* in, int dtype, void* out, float* scal
 int moe_gg_fp8_block128_quant(const void* in, int dtype, void* out, float* scales, int64_t rows, int K, void* stream);
 
 /*
+ * Router gate: the k best experts of a row and the weights of their rows in the layer's sum, and its gradient. The
+ * weights are what combine_topk and the layer take (the reference's test makes them with softmax and topk in torch,
+ * kernels/triton/inference/col_major_moe_gemm/test_moe_gemm.py:54-57).
+ *   p = softmax(logits) over the row, or sigmoid(logits) (score); ids = the k largest logits of the row, descending, ties to
+ *   the lower id, NaN below every number; weights[t, j] = scale * p[t, ids[t, j]], with renormalize != 0 divided by the sum
+ *   of the chosen p. A row whose chosen logits are all -infinity has weights (and gradients) of zero.
+ *   logits device [T, E] (dtype: fp32, bf16 or fp16); weights device out fp32 [T, k]; ids device out int32 [T, k]
+ * Backward: grad_weights device fp32 [T, k], logits and ids as above, grad_logits device out [T, E] in the logits' type. An id
+ * outside [0, E) takes no part; an id named twice counts twice.
+ * E <= MOE_GG_MAX_ROUTE_EXPERTS, k <= min(E, 64), T <= 2^24. fp32 arithmetic.
+ */
+#define MOE_GG_GATE_SOFTMAX 0
+#define MOE_GG_GATE_SIGMOID 1
+int moe_gg_route_gate(const void* logits, int dtype, int64_t T, int E, int k, int score, int renormalize, float scale,
+                      float* weights, int32_t* ids, void* stream);
+int moe_gg_route_gate_backward(const float* grad_weights, const void* logits, int dtype, const int32_t* ids, int64_t T, int E, int k,
+                               int score, int renormalize, float scale, void* grad_logits, void* stream);
+
+/*
+ * Norms before and after a block, fused with the block's gate and the residual sum (no counterpart in the reference; the
+ * element-wise side of a layer whose expert products are above).
+ *   n = y / sqrt(mean(y^2) + eps) * w_post             (w_post null: n = y)
+ *   h = residual_scale * residual + block_scale * gate * n
+ *   z = h / sqrt(mean(h^2) + eps) * w_pre              (w_pre null: no z)
+ * y null: h is not written and z is the norm of the residual as it is (residual_scale must be 1).
+ *   y, z device [T, d] bf16 or fp16 (dtype); residual, h device [T, d] in that type or fp32 (stream_dtype);
+ *   w_post, w_pre device [d], gate device [d] (gate_kind = MOE_GG_GATE_CHANNEL) or [T] (MOE_GG_GATE_ROW), all in dtype or
+ *   fp32 (weight_dtype); ldy, ldr: elements between rows; h and z are contiguous. h may be the residual's memory, z y's.
+ * fp32 arithmetic, one rounding per output. d <= MOE_GG_MAX_NORM_WIDTH, T <= 2^21.
+ * Backward: h the stored sum (the residual where y is null), grad_h (null: zeros) and grad_z the gradients of both outputs;
+ * grad_y [T, d], grad_residual [T, d], grad_w_post, grad_w_pre, grad_gate like their tensors. Outputs that belong to an absent
+ * input are null. No two of the outputs and no output and input share memory, but grad_residual may be grad_h's and
+ * grad_y grad_z's. workspace: moe_gg_block_norm_backward_workspace bytes, 256-byte aligned. Sums over rows are taken
+ * in a fixed order.
+ */
+#define MOE_GG_MAX_NORM_WIDTH 16384
+#define MOE_GG_GATE_NONE 0
+#define MOE_GG_GATE_CHANNEL 1
+#define MOE_GG_GATE_ROW 2
+int moe_gg_block_norm(const void* y, int64_t ldy, const void* residual, int64_t ldr, const void* w_post, const void* gate,
+                      int gate_kind, const void* w_pre, float residual_scale, float block_scale, float eps, void* h, void* z,
+                      int64_t T, int d, int dtype, int stream_dtype, int weight_dtype, void* stream);
+size_t moe_gg_block_norm_backward_workspace(int64_t T, int d);
+int moe_gg_block_norm_backward(const void* grad_h, int64_t ldgh, const void* grad_z, int64_t ldgz, const void* y, int64_t ldy, const void* h,
+                               int64_t ldh, const void* w_post, const void* gate, int gate_kind, const void* w_pre,
+                               float residual_scale, float block_scale, float eps, void* grad_y, void* grad_residual, void* grad_w_post,
+                               void* grad_gate, void* grad_w_pre, int64_t T, int d, int dtype, int stream_dtype, int weight_dtype,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Low-rank adapters of many requests beside one shared projection, and their gradients (no counterpart in the reference;
+ * products grouped by an id per row, like the expert products above). Row t names adapter e = ids[t]:
+ *   h[t] = a[e] x[t]                out[t] = y[t] + scales[e] b[e] h[t]         (rows without an adapter: out[t] = y[t])
+ *   u[t] = scales[e] b[e]^T grad_out[t]
+ *   grad_x[t] = grad_x_in[t] + a[e]^T u[t]      grad_a[e] = sum_t u[t] x[t]^T      grad_b[e] = scales[e] sum_t grad_out[t] h[t]^T
+ * moe_gg_lora_plan groups the rows once for all projections that a batch passes: perm device out int32 [T], the rows of
+ * adapter 0, 1, ... in their order and then the rows whose id lies outside [0, L); offsets device out int32 [L + 2], where
+ * the groups begin and end; scratch device int32 [T + L + 1]. The products below take perm and offsets on the device; entries
+ * that name no row are skipped, so no table can make them leave the tensors.
+ *   x device [T, K], y / out / grad_out device [T, N], grad_x_in / grad_x device [T, K] with their leading dimensions;
+ *   a device [L, R, K], b device [L, N, R] contiguous; grad_a, grad_b like them, zeros for an adapter without rows; all of one
+ *   16-bit type (dtype); scales device fp32 [L] or null (1); h device fp32 [T, R] or null: written by the forward pass (zeros
+ *   in rows without an adapter), read by the backward pass, which computes it again from x where it is null;
+ *   grad_x_in null: zeros. out may be y, grad_x may be grad_x_in (same leading dimension); other tensors must not overlap.
+ * fp32 accumulation; h and u are fp32 and reach the matrix instructions as two 16-bit parts; each output is rounded once. The
+ * order of every sum is fixed by the arguments. a and b must be finite.
+ * R <= MOE_GG_MAX_LORA_RANK, L <= MOE_GG_MAX_LORA_ADAPTERS, T <= 2^20, K and N <= 2^17. workspace: moe_gg_lora_*_workspace bytes, 256-byte aligned; nothing in
+ * it has to survive a call.
+ */
+#define MOE_GG_MAX_LORA_RANK 128
+#define MOE_GG_MAX_LORA_ADAPTERS 767
+int moe_gg_lora_plan(const int32_t* ids, int64_t T, int L, int32_t* perm, int32_t* offsets, int32_t* scratch, void* stream);
+size_t moe_gg_lora_add_workspace(int64_t T, int L, int K, int N, int R);
+int moe_gg_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, const void* a, const void* b, const float* scales,
+                    const int32_t* perm, const int32_t* offsets, int L, int64_t T, int K, int N, int R, void* out, int64_t ldo,
+                    float* h, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t moe_gg_lora_backward_workspace(int64_t T, int L, int K, int N, int R, int with_h);
+int moe_gg_lora_backward(const void* grad_out, int64_t ldg, const void* x, int64_t ldx, const void* a, const void* b, const float* scales,
+                         const int32_t* perm, const int32_t* offsets, int L, int64_t T, int K, int N, int R, const float* h,
+                         const void* grad_x_in, int64_t ld_in, void* grad_x, int64_t ld_grad_x, void* grad_a, void* grad_b, int dtype,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Test / tuning hooks (no counterpart in the reference).
  * moe_gg_set_variant pins the kernel variant used by an op (-1 = automatic choice). The pin is one process-global
  * setting per op (an atomic int): it applies to every later call of that op from any thread, on any device and

@@ -18,6 +18,9 @@ from . import _lib
 from . import ops as _ops
 
 
+_TYPES = (torch.bfloat16, torch.float16)
+
+
 class LoraPlan(NamedTuple):
     """The rows of a batch grouped by adapter: perm [T] int32 holds the rows of adapter 0, 1, ... in their order and then
     the rows without an adapter, offsets [L + 2] int32 where each group begins (the last entry is T)."""
@@ -37,7 +40,7 @@ def lora_plan(adapter_ids: torch.Tensor, num_adapters: int) -> LoraPlan:
     perm = torch.empty((T,), dtype=torch.int32, device=dev)
     offsets = torch.empty((num_adapters + 2,), dtype=torch.int32, device=dev)
     scratch = torch.empty((T + num_adapters + 1,), dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
+    with _ops._on_device(dev):
         rc = _lib.lib().moe_gg_lora_plan(ids.data_ptr(), T, num_adapters, perm.data_ptr(), offsets.data_ptr(), scratch.data_ptr(), _ops._stream_ptr(dev))
     _lib.check(rc, "moe_gg_lora_plan")
     return LoraPlan(perm, offsets)
@@ -48,27 +51,28 @@ def _check(rows: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor
     if x.dim() != 2 or rows.dim() != 2 or a.dim() != 3 or b.dim() != 3:
         raise ValueError(f"{what} and x must be [T, N] and [T, K], a [L, R, K], b [L, N, R]")
     T, K = x.shape
-    L, R, _ = a.shape
-    N = b.shape[1]
-    if a.shape[2] != K or b.shape != (L, N, R) or rows.shape != (T, N):
+    L, R, k = a.shape
+    l, N, r = b.shape
+    if k != K or l != L or r != R or rows.shape != (T, N):
         raise ValueError(f"shapes do not match: {what} {tuple(rows.shape)}, x {tuple(x.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)}")
-    if x.dtype not in (torch.bfloat16, torch.float16) or rows.dtype != x.dtype or a.dtype != x.dtype or b.dtype != x.dtype:
+    dtype = x.dtype
+    if dtype not in _TYPES or rows.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
         raise ValueError(f"{what}, x, a and b must all be bf16 or all be fp16")
-    if plan.perm.shape != (T,) or plan.offsets.shape != (L + 2,) or plan.perm.dtype != torch.int32 or plan.offsets.dtype != torch.int32:
+    perm, offsets = plan
+    if perm.shape != (T,) or offsets.shape != (L + 2,) or perm.dtype != torch.int32 or offsets.dtype != torch.int32:
         raise ValueError(f"the plan is not one of {T} rows and {L} adapters")
-    if not (a.is_contiguous() and b.is_contiguous() and plan.perm.is_contiguous() and plan.offsets.is_contiguous()):
+    if not (a.is_contiguous() and b.is_contiguous() and perm.is_contiguous() and offsets.is_contiguous()):
         raise ValueError("a, b and the plan must be contiguous")
-    tensors = (rows, x, a, b, plan.perm, plan.offsets)
-    if scales is not None:
-        if scales.shape != (L,) or scales.dtype != torch.float32 or not scales.is_contiguous():
-            raise ValueError(f"scales must be contiguous fp32 [{L}]")
-        tensors += (scales,)
-    return _ops._require_cuda(*tensors), L, T, K, N, R
+    if scales is None:
+        return _ops._require_cuda(rows, x, a, b, perm, offsets), L, T, K, N, R
+    if scales.shape != (L,) or scales.dtype != torch.float32 or not scales.is_contiguous():
+        raise ValueError(f"scales must be contiguous fp32 [{L}]")
+    return _ops._require_cuda(rows, x, a, b, perm, offsets, scales), L, T, K, N, R
 
 
 def _row_major(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy, with neighbouring elements of a row next to each other and rows that do not overlap."""
-    return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
+    return t if t.is_contiguous() or (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -77,7 +81,7 @@ def _ld(t: torch.Tensor) -> int:
 
 def _result(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or _row_major(out) is not out:
         raise ValueError(f"{name} must be a row-major tensor of shape {tuple(like.shape)} and {like.dtype} on the inputs' device")
     return out
@@ -95,10 +99,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     if not inplace:
         y = _row_major(y)
     out = _result(out, y, "out")
-    h = torch.empty((T, R), dtype=torch.float32, device=dev) if return_h else None
+    h = x.new_empty((T, R), dtype=torch.float32) if return_h else None
     lib = _lib.lib()
     nbytes = lib.moe_gg_lora_add_workspace(T, L, K, N, R)
-    with torch.cuda.device(dev):
+    with _ops._on_device(dev):
         workspace = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=dev)
         rc = lib.moe_gg_lora_add(y.data_ptr(), _ld(y), x.data_ptr(), _ld(x), a.data_ptr(), b.data_ptr(), None if scales is None else scales.data_ptr(),
                                  plan.perm.data_ptr(), plan.offsets.data_ptr(), L, T, K, N, R, out.data_ptr(), _ld(out),
@@ -131,7 +135,7 @@ def lora_backward(grad_out: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: t
     grad_a, grad_b = torch.empty_like(a), torch.empty_like(b)
     lib = _lib.lib()
     nbytes = lib.moe_gg_lora_backward_workspace(T, L, K, N, R, 0 if h is None else 1)
-    with torch.cuda.device(dev):
+    with _ops._on_device(dev):
         workspace = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=dev)
         rc = lib.moe_gg_lora_backward(grad_out.data_ptr(), _ld(grad_out), x.data_ptr(), _ld(x), a.data_ptr(), b.data_ptr(),
                                       None if scales is None else scales.data_ptr(), plan.perm.data_ptr(), plan.offsets.data_ptr(), L, T, K, N, R,

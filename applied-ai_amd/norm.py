@@ -15,10 +15,11 @@ from . import ops as _ops
 
 _DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # MOE_GG_DTYPE_BF16 / _FP16 / _FP32
 _NONE, _CHANNEL, _ROW = 0, 1, 2                                    # MOE_GG_GATE_*
+_TYPES = (torch.bfloat16, torch.float16)
 
 
 def _row_major(t: torch.Tensor) -> torch.Tensor:
-    return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
+    return t if t.is_contiguous() or (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -34,25 +35,30 @@ def _check(y, stream, post_weight, gate, pre_weight, extra=()):
     if stream.dim() != 2:
         raise ValueError("the residual stream must be [T, d]")
     T, d = stream.shape
+    tensors = [stream]
     if y is not None:
-        if y.shape != stream.shape or y.dtype not in (torch.bfloat16, torch.float16):
+        if y.shape != stream.shape or y.dtype not in _TYPES:
             raise ValueError("the block's output must be bf16 or fp16 of the residual stream's shape")
         if stream.dtype not in (y.dtype, torch.float32):
             raise ValueError("the residual stream must have the block output's type or be fp32")
+        tensors.append(y)
     kind = _NONE
     if gate is not None:
         kind = _CHANNEL if gate.shape == (d,) else _ROW if gate.shape == (T, 1) else -1
         if kind < 0:
             raise ValueError(f"the gate must be [{d}] (per channel) or [{T}, 1] (per row)")
-    small = [t for t in (post_weight, gate, pre_weight) if t is not None]
-    for t in (post_weight, pre_weight):
-        if t is not None and t.shape != (d,):
+    wt = None
+    for t in (post_weight, gate, pre_weight):
+        if t is None:
+            continue
+        if t is not gate and t.shape != (d,):
             raise ValueError(f"a norm's weight must be [{d}]")
-    for t in small:
-        if t.dtype != small[0].dtype or not t.is_contiguous():
+        wt = wt or t.dtype
+        if t.dtype != wt or not t.is_contiguous():
             raise ValueError("the norms' weights and the gate must be contiguous and of one type")
-    tensors = [stream] + ([y] if y is not None else []) + small + [t for t in extra if t is not None]
-    return _ops._require_cuda(*tensors), kind, small[0].dtype if small else None
+        tensors.append(t)
+    tensors += [t for t in extra if t is not None]
+    return _ops._require_cuda(*tensors), kind, wt
 
 
 def block_norm(y: torch.Tensor, residual: torch.Tensor, post_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
@@ -70,9 +76,9 @@ def block_norm(y: torch.Tensor, residual: torch.Tensor, post_weight: Optional[to
         raise ValueError("weights and gate must have the block output's type or be fp32")
     y, residual = _row_major(y), _row_major(residual)
     T, d = y.shape
-    h = torch.empty((T, d), dtype=residual.dtype, device=dev)
-    z = torch.empty((T, d), dtype=y.dtype, device=dev) if pre_weight is not None else None
-    with torch.cuda.device(dev):
+    h = torch.empty_like(residual, memory_format=torch.contiguous_format)
+    z = torch.empty_like(y, memory_format=torch.contiguous_format) if pre_weight is not None else None
+    with _ops._on_device(dev):
         rc = _lib.lib().moe_gg_block_norm(y.data_ptr(), _ld(y), residual.data_ptr(), _ld(residual), _ptr(post_weight), _ptr(gate), kind, _ptr(pre_weight),
                                           residual_scale, block_scale, eps, h.data_ptr(), _ptr(z), T, d, _DTYPE[y.dtype], _DTYPE[residual.dtype],
                                           _DTYPE[wt or y.dtype], _ops._stream_ptr(dev))
@@ -105,12 +111,12 @@ def _backward(grad_h, grad_z, y, h, post_weight, gate, pre_weight, residual_scal
         raise ValueError(f"grad_h must be {h.dtype} {tuple(h.shape)}")
     T, d = h.shape
     y, h, grad_h, grad_z = (None if t is None else _row_major(t) for t in (y, h, grad_h, grad_z))
-    grad_y = None if y is None else torch.empty((T, d), dtype=dtype, device=dev)
-    grad_residual = torch.empty((T, d), dtype=h.dtype, device=dev)
+    grad_y = None if y is None else torch.empty_like(y, memory_format=torch.contiguous_format)
+    grad_residual = torch.empty_like(h, memory_format=torch.contiguous_format)
     grad_post, grad_gate, grad_pre = (None if t is None else torch.empty_like(t) for t in (post_weight, gate, pre_weight))
     lib = _lib.lib()
     nbytes = lib.moe_gg_block_norm_backward_workspace(T, d)
-    with torch.cuda.device(dev):
+    with _ops._on_device(dev):
         workspace = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=dev)
         rc = lib.moe_gg_block_norm_backward(_ptr(grad_h), 0 if grad_h is None else _ld(grad_h), _ptr(grad_z), 0 if grad_z is None else _ld(grad_z),
                                             _ptr(y), 0 if y is None else _ld(y), h.data_ptr(), _ld(h), _ptr(post_weight), _ptr(gate), kind,
@@ -133,8 +139,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, dtype: Op
         raise ValueError("the weight must have the result's type or be fp32")
     x = _row_major(x)
     T, d = x.shape
-    z = torch.empty((T, d), dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
+    z = x.new_empty((T, d), dtype=dtype)
+    with _ops._on_device(dev):
         rc = _lib.lib().moe_gg_block_norm(None, 0, x.data_ptr(), _ld(x), None, None, _NONE, weight.data_ptr(), 1.0, 1.0, eps, None, z.data_ptr(), T, d,
                                           _DTYPE[dtype], _DTYPE[x.dtype], _DTYPE[wt], _ops._stream_ptr(dev))
     if rc:

@@ -4,6 +4,7 @@ Same names, argument meaning and return values as the reference launchers; the w
 hand-written gfx950 kernels behind the C ABI in include/moe_gg.h. torch is used for device
 memory and the current stream only.
 """
+import contextlib
 from typing import Optional
 
 import torch
@@ -15,12 +16,23 @@ OUT_BLOCK = 1
 
 
 def _stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the handle alone: building a torch.cuda.Stream object around it costs 1.8 us, this 0.1 us
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on_device(device: torch.device):
+    """torch.cuda.device(device), at a fifth of its 1.3 us where that is the current device already."""
+    return _HERE if device.index is not None and torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _require_cuda(*tensors: torch.Tensor) -> torch.device:
     dev = tensors[0].device
     for t in tensors:
+        if t.is_cuda and t.device == dev:
+            continue
         if t.device.type != "cuda":
             raise RuntimeError(
                 "applied_ai_amd ops run on a HIP device only (got a %s tensor); there is no CPU path"

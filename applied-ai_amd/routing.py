@@ -9,7 +9,7 @@ from typing import Tuple
 import torch
 
 from . import _lib
-from .ops import _require_cuda, _stream_ptr
+from .ops import _on_device, _require_cuda, _stream_ptr
 
 
 def route_topk(logits: torch.Tensor, k: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -118,9 +118,9 @@ def route_gate(logits: torch.Tensor, k: int, score: str = "softmax", renormalize
     dev = _require_cuda(logits)
     logits = logits.contiguous()
     T, E = logits.shape
-    weights = torch.empty((T, k), dtype=torch.float32, device=dev)
-    ids = torch.empty((T, k), dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
+    weights = logits.new_empty((T, k), dtype=torch.float32)
+    ids = logits.new_empty((T, k), dtype=torch.int32)
+    with _on_device(dev):
         rc = _lib.lib().moe_gg_route_gate(logits.data_ptr(), _LOGITS[logits.dtype], T, E, k, _SCORES[score], 1 if renormalize else 0, scale,
                                           weights.data_ptr(), ids.data_ptr(), _stream_ptr(dev))
     if rc:
@@ -140,8 +140,8 @@ def route_gate_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids: t
     dev = _require_cuda(grad_weights, logits, ids)
     grad_weights, logits, ids = grad_weights.contiguous(), logits.contiguous(), ids.contiguous()
     T, E = logits.shape
-    grad = torch.empty((T, E), dtype=logits.dtype, device=dev)
-    with torch.cuda.device(dev):
+    grad = torch.empty_like(logits)
+    with _on_device(dev):
         rc = _lib.lib().moe_gg_route_gate_backward(grad_weights.data_ptr(), logits.data_ptr(), _LOGITS[logits.dtype], ids.data_ptr(), T, E, ids.shape[1],
                                                    _SCORES[score], 1 if renormalize else 0, scale, grad.data_ptr(), _stream_ptr(dev))
     if rc:

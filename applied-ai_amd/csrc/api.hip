@@ -894,7 +894,7 @@ int moe_gg_lora_add(const void* y, int64_t ldy, const void* x, int64_t ldx, cons
   if (dtype != MOE_GG_DTYPE_BF16 && dtype != MOE_GG_DTYPE_FP16) return MOE_GG_EINVAL;
   if (T == 0) return MOE_GG_OK;
   if (ldy < N || ldo < N || ldx < K || (out == y && ldo != ldy)) return MOE_GG_ESHAPE;
-  if (!y || !x || !out || !perm || !offsets || (L > 0 && (!a || !b)) || !workspace) return MOE_GG_EINVAL;
+  if (!y || !x || !out || !perm || !offsets || (L > 0 && (!a || !b)) || (!workspace && workspace_bytes)) return MOE_GG_EINVAL;
   if (!aligned(y, 2) || !aligned(x, 2) || !aligned(out, 2) || !aligned(a, 2) || !aligned(b, 2) || !aligned(scales, 4) || !aligned(h, 4) ||
       !aligned(perm, 4) || !aligned(offsets, 4) || !aligned(workspace, 256))
     return MOE_GG_EALIGN;

@@ -4,18 +4,22 @@
 //   h[t] = A_e x[t]                     out[t] = y[t] + s_e B_e h[t]                 (rows without an adapter: out = y)
 //   u[t] = s_e B_e^T gout[t]            gx[t] = gx_in[t] + A_e^T u[t]
 //   gA_e = sum_t u[t] x[t]^T            gB_e = s_e sum_t gout[t] h[t]^T
-// The rank R is small, so every product moves far more bytes than it computes: x, y, out, gout, gx pass once per kernel and
+// The rank R is small, so every product moves far more bytes than it computes: x, y, out, gout, gx pass through the kernels and
 // the matrix instructions only keep up with memory. Three kernels do all of it:
 //   shrink  [rows, C] . [R, C]^T  -> [rows, R]   the long axis C is reduced: split over workgroups and waves
 //   expand  [rows, R] . [C, R]^T  -> [rows, C]   added to a row of y on its way through
-//   wgrad   [rows, C]^T . [rows, R] -> [C, R]    rows are reduced, adapter by adapter
-// and the backward pass runs shrink and expand on transposed copies of B and A (R x C each, small beside the rows).
+//   wgrad   [rows, C]^T . [rows, R] -> [C, R]    rows are reduced, adapter by adapter; on the output's gradient it also takes
+//                                                the product with B (u) from the same rows, which are then read once
+// and for a few rows shrink and expand are one kernel without an intermediate in memory.
 //
 // Rows are taken in adapter order (perm, offsets of the plan). Group g = adapter g for g < L and "no adapter" for g = L.
 // A grid cannot know the groups' sizes without a copy to the host, so it counts slots of `unit` rows:
 // group g owns slots [off_g / unit + g, off_{g+1} / unit + g + 1), at least as many as it needs, and a workgroup
 // finds its group with one ballot over the group table (two beyond 64 groups). [rows, R] intermediates live in the same space
 // with unit 16: group g's rows start at 16 * (off_g / 16 + g), so that every group is aligned and padded with zero rows.
+//
+// Where that is fewer, slots are the rows themselves, of which every unit-th of a group has work (a few single tokens beside
+// many loaded adapters).
 //
 // The intermediates are fp32. As matrix operands they are split into a high and a low part of the 16-bit type, which keep
 // 16 (bf16) or 22 (fp16) significant bits: one matrix instruction covers 16 ranks, its 32-deep reduction holding
@@ -28,6 +32,8 @@ namespace {
 
 typedef __attribute__((__vector_size__(2 * sizeof(uint16_t)))) uint16_t u16x2_t;
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
+
+template <int N> struct Number { static constexpr int value = N; };
 
 struct Rows {
   const int32_t* perm;     // [T] rows in group order
@@ -47,33 +53,52 @@ struct Slot {
   int size;    // rows of the group
 };
 
+DEVINL bool slots_are_rows(const Rows& r, int unit) { return r.T < r.T / unit + r.G; }
+DEVINL Slot slot_of(const Rows& r, int v, int unit, int g, int begin, int end) {
+  int skip = (v - (begin / unit + g)) * unit;
+  if (slots_are_rows(r, unit)) skip = (v - begin) % unit == 0 ? v - begin : -1;
+  Slot s;
+  s.begin = begin;
+  s.size = end - begin;
+  s.first = begin + skip;
+  s.rows = min(unit, s.size - skip);
+  s.padded = 16 * (begin / 16 + g) + skip;
+  s.group = s.rows > 0 && skip >= 0 ? g : -1;
+  return s;
+}
 // Which rows slot v of `unit` rows holds. All lanes of the wave take part; the result is the same in all of them. Whatever
 // the table holds, the rows named lie inside [0, T).
 DEVINL Slot find_slot(const Rows& r, int v, int unit) {
   const int lane = lane_id();
+  const bool by_row = slots_are_rows(r, unit);
+  if (r.G < 64) {  // the whole table in one load
+    const int off = clamp_off(r, min(lane, r.G));
+    const int g = min(max(__popcll(__ballot(lane < r.G && (by_row ? off : off / unit + lane) <= v)) - 1, 0), r.G - 1);
+    return slot_of(r, v, unit, g, __shfl(off, g, 64), __shfl(off, g + 1, 64));
+  }
   const int step = (r.G + 63) >> 6;
   int i = lane * step;
-  bool le = i < r.G && clamp_off(r, min(i, r.G)) / unit + i <= v;
+  int off = clamp_off(r, min(i, r.G));
+  bool le = i < r.G && (by_row ? off : off / unit + i) <= v;
   int g = max(__popcll(__ballot(le)) - 1, 0) * step;
   if (step > 1) {
     i = g + lane;
-    le = lane < step && i < r.G && clamp_off(r, min(i, r.G)) / unit + i <= v;
+    off = clamp_off(r, min(i, r.G));
+    le = lane < step && i < r.G && (by_row ? off : off / unit + i) <= v;
     g += max(__popcll(__ballot(le)) - 1, 0);
   }
   g = min(g, r.G - 1);
-  Slot s;
-  s.begin = clamp_off(r, g);
-  s.size = clamp_off(r, g + 1) - s.begin;
-  const int skip = (v - (s.begin / unit + g)) * unit;
-  s.first = s.begin + skip;
-  s.rows = min(unit, s.size - skip);
-  s.padded = 16 * (s.begin / 16 + g) + skip;
-  s.group = s.rows > 0 && skip >= 0 ? g : -1;
-  return s;
+  return slot_of(r, v, unit, g, clamp_off(r, g), clamp_off(r, g + 1));
 }
 
-DEVINL u32x4_t load16(const uint16_t* p) { return *(const u32x4_t*)p; }
-// Eight elements p[0..7] of which only the first n exist; no alignment.
+// Eight elements at any address: the hardware's wide loads and stores need no alignment, and what an unaligned one costs
+// is the second line that it may touch.
+typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
+typedef u32x2_t u32x2_any_t __attribute__((aligned(2)));
+typedef f32x4_t f32x4_any_t __attribute__((aligned(4)));
+DEVINL u32x4_t load16(const uint16_t* p) { return *(const u32x4_any_t*)p; }
+DEVINL void store16(uint16_t* p, u32x4_t v) { *(u32x4_any_t*)p = v; }
+// Eight elements p[0..7] of which only the first n exist (none for n <= 0).
 DEVINL u32x4_t load_some(const uint16_t* p, int n) {
   u32x4_t v = {0u, 0u, 0u, 0u};
 #pragma unroll
@@ -101,8 +126,7 @@ template <bool F16> DEVINL void split16(float v, uint16_t& hi, uint16_t& lo) {
 // ---- shrink -------------------------------------------------------------------------------------------------------------
 // part[split][padded row][r] = sum over the split's columns of x[row, c] * w[group, r, c].
 // A workgroup takes MF x 16 rows and one split; its eight waves take an eighth of the split each and are summed through LDS.
-// A lane holds 16 consecutive columns of its row as two operands: with the column order changed the same way on both sides
-// the sum is the same, and four lanes read 128 consecutive bytes of a row.
+// A row is read by four lanes, 64 consecutive bytes at a time.
 struct ShrinkParams {
   const uint16_t* x;
   int64_t ldx;
@@ -113,109 +137,133 @@ struct ShrinkParams {
   int C, R, Rp, P, splits, per_wave;  // per_wave: columns per wave, a multiple of 64
 };
 
-template <bool F16, int NF, int MF, bool VEC>
+// acc += the products of columns [k0, k1) of a wave: xr, wr point at column 8 q of this lane's rows, MANY x 64 columns have
+// their loads under way before the first product.
+template <bool F16, int NF, int MF, int MANY>
+DEVINL void shrink_columns(const uint16_t* const (&xr)[MF], const uint16_t* const (&wr)[NF], int k0, int k1, int q, f32x4_t (&acc)[MF][NF]) {
+  auto columns = [&](int k, auto steps) {
+    constexpr int STEPS = decltype(steps)::value;
+    u32x4_t xv[STEPS][2][MF], wv[STEPS][2][NF];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int i = 0; i < MF; ++i) xv[s][b][i] = load16(xr[i] + k + 64 * s + 32 * b);
+#pragma unroll
+        for (int j = 0; j < NF; ++j) wv[s][b][j] = load16(wr[j] + k + 64 * s + 32 * b);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+          for (int j = 0; j < NF; ++j) acc[i][j] = mfma_16x16x32<F16>(xv[s][b][i], wv[s][b][j], acc[i][j]);
+  };
+  for (; k0 + 64 * MANY <= k1; k0 += 64 * MANY) columns(k0, Number<MANY>());
+  if (MANY > 1)
+    for (; k0 + 64 <= k1; k0 += 64) columns(k0, Number<1>());
+  if (k0 < k1) {  // the last columns of a width that is no multiple of 64
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int n = k1 - (k0 + 8 * q + 32 * b);
+      u32x4_t xv[MF], wv[NF];
+#pragma unroll
+      for (int i = 0; i < MF; ++i) xv[i] = n >= 8 ? load16(xr[i] + k0 + 32 * b) : load_some(xr[i] + k0 + 32 * b, n);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) wv[j] = n >= 8 ? load16(wr[j] + k0 + 32 * b) : load_some(wr[j] + k0 + 32 * b, n);
+      wave_whole();
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] = mfma_16x16x32<F16>(xv[i], wv[j], acc[i][j]);
+    }
+  }
+}
+
+// The operand rows of a lane. Rows that do not exist read an existing one in their place: a result belongs to one row of
+// each operand, and theirs are not kept.
+template <int MF> DEVINL void shrink_rows(const Rows& rows, const Slot& s, const uint16_t* x, int64_t ldx, const uint16_t* (&xr)[MF]) {
+#pragma unroll
+  for (int i = 0; i < MF; ++i) {
+    const int t = rows.perm[s.first + min(16 * i + (lane_id() & 15), s.rows - 1)];
+    xr[i] = x + (int64_t)(t >= 0 && t < rows.T ? t : 0) * ldx + 8 * (lane_id() >> 4);
+  }
+}
+template <int NF> DEVINL void shrink_weights(const Slot& s, const uint16_t* w, int64_t ldw, int R, const uint16_t* (&wr)[NF]) {
+#pragma unroll
+  for (int j = 0; j < NF; ++j) {
+    const int r = 16 * j + (lane_id() & 15);
+    wr[j] = w + ((int64_t)s.group * R + (r < R ? r : 0)) * ldw + 8 * (lane_id() >> 4);
+  }
+}
+
+template <bool F16, int NF, int MF>
 __global__ __launch_bounds__(512) void lora_shrink(ShrinkParams p, int slots) {
-  __shared__ f32x4_t red[4][MF * NF][64];
+  constexpr int WAVES = MF * NF > 8 ? 4 : 8;  // whose sums are in LDS at a time: 64 KB at most
+  __shared__ __align__(16) float red[WAVES][16 * MF][16 * NF];
   const int split = blockIdx.x / slots;
   const Slot s = find_slot(p.rows, blockIdx.x - split * slots, 16 * MF);
   if (s.group < 0 || s.group == p.rows.G - 1) return;
   const int lane = lane_id(), wave = wave_id(), i16 = lane & 15, q = lane >> 4;
-  const int mf = (s.rows + 15) >> 4;
-  // Operand rows that do not exist read row 0 of their matrix: a result belongs to one row of each operand, and theirs are
-  // not kept.
   const uint16_t* xr[MF];
-#pragma unroll
-  for (int i = 0; i < MF; ++i) {
-    const int t = p.rows.perm[s.first + min(16 * i + i16, s.rows - 1)];
-    xr[i] = p.x + (int64_t)(t >= 0 && t < p.rows.T ? t : 0) * p.ldx + 16 * q;
-  }
   const uint16_t* wr[NF];
-#pragma unroll
-  for (int j = 0; j < NF; ++j) {
-    const int r = 16 * j + i16;
-    wr[j] = p.w + ((int64_t)s.group * p.R + (r < p.R ? r : 0)) * p.ldw + 16 * q;
-  }
+  shrink_rows<MF>(p.rows, s, p.x, p.ldx, xr);
+  shrink_weights<NF>(s, p.w, p.ldw, p.R, wr);
   f32x4_t acc[MF][NF];
 #pragma unroll
   for (int i = 0; i < MF; ++i)
 #pragma unroll
     for (int j = 0; j < NF; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  auto multiply = [&](const u32x4_t (&xv)[MF][2], const u32x4_t (&wv)[NF][2]) {
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < MF; ++i)
-#pragma unroll
-        for (int j = 0; j < NF; ++j) acc[i][j] = mfma_16x16x32<F16>(xv[i][b], wv[j][b], acc[i][j]);
-  };
   const int64_t begin = (int64_t)(split * 8 + wave) * p.per_wave;
-  const int k1 = (int)min((int64_t)p.C, begin + p.per_wave);
-  int k0 = (int)min(begin, (int64_t)p.C);
-  if (VEC)
-    for (; k0 + 64 <= k1; k0 += 64) {
-      u32x4_t xv[MF][2], wv[NF][2];
+  shrink_columns<F16, NF, MF, (MF + NF <= 2 ? 2 : 1)>(xr, wr, (int)min(begin, (int64_t)p.C), (int)min((int64_t)p.C, begin + p.per_wave), q, acc);
+  auto put = [&](int w) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-#pragma unroll
-        for (int j = 0; j < NF; ++j) wv[j][b] = load16(wr[j] + k0 + 8 * b);
-#pragma unroll
-        for (int i = 0; i < MF; ++i) xv[i][b] = load16(xr[i] + k0 + 8 * b);
-      }
-      multiply(xv, wv);
-    }
-  for (; k0 < k1; k0 += 64) {
-    u32x4_t xv[MF][2], wv[NF][2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int n = min(8, k1 - (k0 + 16 * q + 8 * b));
-#pragma unroll
-      for (int j = 0; j < NF; ++j) wv[j][b] = load_some(wr[j] + k0 + 8 * b, n);
-#pragma unroll
-      for (int i = 0; i < MF; ++i) xv[i][b] = load_some(xr[i] + k0 + 8 * b, n);
-    }
-    wave_whole();
-    multiply(xv, wv);
-  }
-#pragma unroll
-  for (int half = 4; half >= 1; half >>= 1) {
-    if (wave >= half && wave < 2 * half)
-#pragma unroll
-      for (int i = 0; i < MF; ++i)
-#pragma unroll
-        for (int j = 0; j < NF; ++j) red[wave - half][i * NF + j][lane] = acc[i][j];
-    __syncthreads();
-    if (wave < half)
-#pragma unroll
-      for (int i = 0; i < MF; ++i)
-#pragma unroll
-        for (int j = 0; j < NF; ++j) acc[i][j] += red[wave][i * NF + j][lane];
-    __syncthreads();
-  }
-  if (wave != 0) return;
-  float* out = p.part + ((int64_t)split * p.P + s.padded) * p.Rp;
-#pragma unroll
-  for (int i = 0; i < MF; ++i)
-    if (i < mf)
+    for (int i = 0; i < MF; ++i)
 #pragma unroll
       for (int j = 0; j < NF; ++j)
-        if (16 * j < p.Rp)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int n = 16 * i + 4 * q + e, r = 16 * j + i16;
-            out[(int64_t)n * p.Rp + r] = n < s.rows && r < p.R ? acc[i][j][e] : 0.f;
-          }
+        for (int e = 0; e < 4; ++e) red[w][16 * i + 4 * q + e][16 * j + i16] = acc[i][j][e];
+  };
+  if (WAVES == 4) {
+    if (wave >= 4) put(wave - 4);
+    __syncthreads();
+    if (wave < 4)
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] += red[wave][16 * i + 4 * q + e][16 * j + i16];
+  }
+  if (wave < WAVES) put(wave);
+  __syncthreads();
+  float* out = p.part + ((int64_t)split * p.P + s.padded) * p.Rp;
+  for (int n = threadIdx.x; n < 64 * MF * NF; n += 512) {  // four ranks of a row
+    const int row = n / (4 * NF), r = 4 * (n % (4 * NF));
+    if (row >= ((s.rows + 15) & ~15) || r >= p.Rp) continue;
+    f32x4_t v = *(const f32x4_t*)&red[0][row][r];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) v += *(const f32x4_t*)&red[w][row][r];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (row >= s.rows || r + e >= p.R) v[e] = 0.f;
+    *(f32x4_t*)(out + (int64_t)row * p.Rp + r) = v;
+  }
 }
 
 // ---- expand -------------------------------------------------------------------------------------------------------------
 // out[row, c] = y[row, c] + s_g sum_r h[row, r] w[group, c, r], h the sum of the splits' parts. A workgroup takes MF x 16
-// rows and `cols` columns: h goes to LDS once as [high | low] operands, then every wave takes strips of 64 columns. Of a
-// strip, operand row i of fragment j is column 16 (i / 4) + 4 j + i % 4, so a lane's results are 16 consecutive columns of one row.
+// rows and `cols` columns: h goes to LDS once as [high | low] operands, every wave takes strips of 64 columns. Of a
+// strip, operand row i of fragment j is column 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4: a lane's results are twice eight
+// consecutive columns of one row, and the four lanes of a row store 64 consecutive bytes.
+// WT: w is [group, r, c] (the backward pass with A): a strip of it goes through the wave's LDS and is read back transposed.
 struct ExpandParams {
   const float* part;
-  const uint16_t* w;  // [L, C, ldw], elements beyond R of a row are not read unless wvec (then they are zero)
-  int64_t ldw;
-  int wvec;           // rows of w are whole 16-byte pieces
+  const uint16_t* w;  // [L, C, R], WT: [L, R, C]
   const float* scales;
   const uint16_t* y;  // may be null: zeros
   int64_t ldy;
@@ -226,33 +274,176 @@ struct ExpandParams {
   int C, R, Rp, P, splits, cols;
 };
 
-template <bool F16, int KF, int MF, bool VEC>
-__global__ __launch_bounds__(256) void lora_expand(ExpandParams p, int slots) {
-  __shared__ __align__(16) uint16_t hs[KF][16 * MF][32];
-  __shared__ float row_up[16 * MF];
-  __shared__ int row_t[16 * MF];
-  const int block = blockIdx.x / slots;
-  const Slot s = find_slot(p.rows, blockIdx.x - block * slots, 16 * MF);
-  if (s.group < 0) return;
-  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), i16 = lane & 15, q = lane >> 4;
-  const bool none = s.group == p.rows.G - 1;
-  const float scale = none ? 0.f : p.scales ? p.scales[s.group] : 1.f;
-  const int mf = (s.rows + 15) >> 4;
-  if (tid < 16 * MF) {
-    const int t = tid < s.rows ? p.rows.perm[s.first + tid] : -1;
-    row_t[tid] = t < p.rows.T ? t : -1;
+// Four rows of 16 columns per 16 lanes, read transposed from LDS: lane i gets column i of rows 0..3 at `at` and of the four
+// rows `next` bytes on. A lane's address is row (i / 4)'s, four columns at (i % 4)'s place.
+DEVINL u32x4_t read_transposed(const uint16_t* at, uint32_t next) {
+  typedef __attribute__((address_space(3))) i16x4_t* lds_ptr;
+  const uint32_t a = (uint32_t)(uintptr_t)at;
+  const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(uintptr_t)a);
+  const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(uintptr_t)(a + next));
+  const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
+  return u32x4_t{l2[0], l2[1], h2[0], h2[1]};
+}
+
+// The rows of a lane (operand column i16 of each fragment), -1 where there is none.
+template <int MF> DEVINL void lane_rows(const Rows& rows, const Slot& s, int (&t)[MF]) {
+#pragma unroll
+  for (int i = 0; i < MF; ++i) {
+    const int n = 16 * i + (lane_id() & 15);
+    t[i] = n < s.rows ? rows.perm[s.first + n] : -1;
+    if (t[i] >= rows.T) t[i] = -1;
   }
-  __syncthreads();
-  // four ranks of a row per thread; the KF * 4 threads of a row are neighbours in a wave
-  for (int n = tid; n < 16 * MF * KF * 4; n += 256) {
+}
+
+constexpr int WT_ROW = 72;  // elements from rank to rank of a transposed strip in LDS
+
+// A strip of 64 columns of a wave: what it reads, and what it makes of it.
+template <bool F16, int KF, int MF, bool WT>
+struct Strip {
+  u32x4_t y[MF][2], w[KF][4];
+
+  // EDGE: the strip reaches beyond the last column (a case of its own, to keep what every strip runs through short)
+  DEVINL void load(const ExpandParams& p, int group, bool none, const int (&t)[MF], int c0) {
+    if (c0 + 64 <= p.C) load<false>(p, group, none, t, c0);
+    else load<true>(p, group, none, t, c0);
+  }
+  // rows and columns that do not exist read existing ones: their results are not stored
+  template <bool EDGE> DEVINL void load(const ExpandParams& p, int group, bool none, const int (&t)[MF], int c0) {
+    const int i16 = lane_id() & 15, q = lane_id() >> 4, c = c0 + 8 * q;
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) y[i][b] = u32x4_t{0u, 0u, 0u, 0u};
+    if (p.y)
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        const uint16_t* src = p.y + (int64_t)max(t[i], 0) * p.ldy + c;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int n = p.C - c - 32 * b;
+          if (!EDGE || n >= 8) y[i][b] = load16(src + 32 * b);
+          else y[i][b] = load_some(src + 32 * b, n);
+        }
+      }
+#pragma unroll
+    for (int k = 0; k < KF; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[k][j] = u32x4_t{0u, 0u, 0u, 0u};
+    if (none) return;
+    if (WT) {
+      // 2 KF pieces of eight ranks x 64 columns: rank lane / 8, columns 8 (lane % 8)
+#pragma unroll
+      for (int k = 0; k < 2 * KF; ++k) {
+        const int r = 8 * k + (lane_id() >> 3), cw = c0 + 8 * (lane_id() & 7), n = r < p.R ? p.C - cw : 0;
+        const uint16_t* src = p.w + ((int64_t)group * p.R + r) * p.C + cw;
+        if (EDGE ? n >= 8 : r < p.R) w[k >> 2][k & 3] = load16(src);
+        else if (EDGE && n > 0) w[k >> 2][k & 3] = load_some(src, n);
+      }
+    } else {
+      const bool whole = p.R % 8 == 0;
+#pragma unroll
+      for (int k = 0; k < KF; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int cw = min(c0 + 32 * (j >> 1) + 8 * (i16 >> 2) + 4 * (j & 1) + (i16 & 3), p.C - 1), r = 16 * k + 8 * (q & 1);
+          const uint16_t* src = p.w + ((int64_t)group * p.C + cw) * p.R + r;
+          if (whole) w[k][j] = r < p.R ? load16(src) : w[k][j];
+          else w[k][j] = r + 8 <= p.R ? load16(src) : load_some(src, p.R - r);
+        }
+    }
+  }
+
+  // WT: from the loaded pieces to operands, through `tile` [16 KF][WT_ROW], which is this wave's alone
+  DEVINL void transpose(uint16_t* tile) {
+    const int i16 = lane_id() & 15, q = lane_id() >> 4;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int k = 0; k < 2 * KF; ++k) *(u32x4_t*)(tile + (8 * k + (lane_id() >> 3)) * WT_ROW + 8 * (lane_id() & 7)) = w[k >> 2][k & 3];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int k = 0; k < KF; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[k][j] = read_transposed(tile + (16 * k + 8 * (q & 1) + (i16 >> 2)) * WT_ROW + 32 * (j >> 1) + 8 * (i16 & 3) + 4 * (j & 1), 4 * WT_ROW * 2);
+  }
+
+  template <class H> DEVINL void finish(const ExpandParams& p, bool none, const int (&t)[MF], int c0, const H& hs, const float* row_up) {
+    if (c0 + 64 <= p.C) finish<false>(p, none, t, c0, hs, row_up);
+    else finish<true>(p, none, t, c0, hs, row_up);
+  }
+  template <bool EDGE, class H> DEVINL void finish(const ExpandParams& p, bool none, const int (&t)[MF], int c0, const H& hs, const float* row_up) {
+    const int i16 = lane_id() & 15, q = lane_id() >> 4, c = c0 + 8 * q;
+    wave_whole();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+      f32x4_t acc[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KF; ++k) {
+        const u32x4_t hv = *(const u32x4_t*)&hs[k][16 * i + i16][8 * q];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = mfma_16x16x32<F16>(w[k][j], hv, acc[j]);
+      }
+      const float up = row_up[16 * i + i16];
+      if (t[i] >= 0) {
+        uint16_t* dst = p.out + (int64_t)t[i] * p.ldo + c;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          u32x4_t o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // columns 32 b + 8 q + 2 e and the next one: fragment 2 b + e / 2, results 2 (e % 2) and the next one
+            const float v0 = f32_of_16<F16>((uint16_t)(y[i][b][e] & 0xFFFFu)), v1 = f32_of_16<F16>((uint16_t)(y[i][b][e] >> 16));
+            const f32x4_t& a = acc[2 * b + (e >> 1)];
+            o[e] = none ? y[i][b][e] : pack_16x2<F16>(v0 + up * a[2 * (e & 1)], v1 + up * a[2 * (e & 1) + 1]);
+          }
+          const int n = p.C - c - 32 * b;
+          if (!EDGE || n >= 8) {
+            store16(dst + 32 * b, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (e < n) dst[32 * b + e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
+          }
+        }
+      }
+      wave_whole();
+    }
+  }
+};
+
+// v[0] + v[step] + ... of `parts` vectors `next` elements apart, in that order; MANY loads are under way at a time.
+template <int MANY> DEVINL f32x4_t sum_parts(const float* part, int parts, int step, int64_t next) {
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < parts; c += MANY * step) {
+    f32x4_t a[MANY];
+#pragma unroll
+    for (int i = 0; i < MANY; ++i) a[i] = *(const f32x4_t*)(part + min(c + i * step, parts - 1) * next);
+#pragma unroll
+    for (int i = 0; i < MANY; ++i)
+      if (c + i * step < parts) v += a[i];
+  }
+  return v;
+}
+
+// h of the workgroup's rows into LDS, from `parts` sums at `part` (rows of Rp, `next` elements from part to part): four ranks
+// of a row per thread; the KF * 4 threads of a row are neighbours in a wave.
+template <bool F16, int KF, int MF, int THREADS, class H>
+DEVINL void put_h(const ExpandParams& p, const Slot& s, bool none, bool write_h, const float* part, int parts, int64_t next, int Rp, H& hs, float* row_up) {
+  const float scale = none ? 0.f : p.scales ? p.scales[s.group] : 1.f;
+  for (int n = threadIdx.x; n < 16 * MF * KF * 4; n += THREADS) {
     const int row = n / (KF * 4), r = (n % (KF * 4)) * 4;
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-    if (!none && row < s.rows && r < p.Rp)
-      for (int c = 0; c < p.splits; ++c) v += *(const f32x4_t*)(p.part + ((int64_t)c * p.P + s.padded + row) * p.Rp + r);
-    if (p.h && block == 0 && row < s.rows && row_t[row] >= 0)
+    if (!none && row < s.rows && r < Rp) v = sum_parts<(MF == 1 ? 8 : 2)>(part + row * Rp + r, parts, 1, next);
+    if (write_h && row < s.rows) {
+      const int t = p.rows.perm[s.first + row];
+      if (t >= 0 && t < p.rows.T)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (r + e < p.R) p.h[(int64_t)row_t[row] * p.R + r + e] = v[e];
+        for (int e = 0; e < 4; ++e)
+          if (r + e < p.R) p.h[(int64_t)t * p.R + r + e] = v[e];
+    }
     float f = 1.f, up = scale;
     if (F16) {
       float m = 0.f;
@@ -277,177 +468,159 @@ __global__ __launch_bounds__(256) void lora_expand(ExpandParams p, int slots) {
     *(u32x2_t*)d = u32x2_t{hi[0], hi[1]};
     *(u32x2_t*)(d + 16) = u32x2_t{lo[0], lo[1]};
   }
-  __syncthreads();
-  if (none && p.out == p.y) return;
+}
 
+template <bool F16, int KF, int MF, bool WT>
+__global__ __launch_bounds__(256) void lora_expand(ExpandParams p, int slots) {
+  __shared__ __align__(16) uint16_t hs[KF][16 * MF][32];
+  __shared__ float row_up[16 * MF];
+  __shared__ __align__(16) uint16_t tiles[WT ? 4 : 1][WT ? 16 * KF : 1][WT_ROW];
+  const int block = blockIdx.x / slots;
+  const Slot s = find_slot(p.rows, blockIdx.x - block * slots, 16 * MF);
+  if (s.group < 0) return;
+  const bool none = s.group == p.rows.G - 1;
   const int64_t c_begin = (int64_t)block * p.cols;
   const int c_end = (int)min((int64_t)p.C, c_begin + p.cols);
-  for (int c0 = (int)c_begin + 64 * wave; c0 < c_end; c0 += 256) {
-    // Columns and rows that do not exist read existing ones in their place: their results are not stored.
-    u32x4_t wv[KF][4];
-#pragma unroll
-    for (int k = 0; k < KF; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = min(c0 + 16 * (i16 >> 2) + 4 * j + (i16 & 3), p.C - 1), r = 16 * k + 8 * (q & 1);
-        const uint16_t* src = p.w + ((int64_t)s.group * p.C + c) * p.ldw;
-        if (none) {
-          wv[k][j] = u32x4_t{0u, 0u, 0u, 0u};
-        } else if (p.wvec) {
-          const u32x4_t v = load16(src + min(r, (int)p.ldw - 8));
-          wv[k][j] = r < p.R ? v : u32x4_t{0u, 0u, 0u, 0u};
-        } else {
-          wv[k][j] = load_some(src + r, p.R - r);
-        }
-      }
-    const int c = c0 + 16 * q;  // this lane's 16 results
-#pragma unroll
-    for (int i = 0; i < MF; ++i) {
-      if (i >= mf) break;
-      const int t = row_t[16 * i + i16];
-      const float up = row_up[16 * i + i16];
-      u32x4_t yv[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        yv[b] = u32x4_t{0u, 0u, 0u, 0u};
-        if (p.y) {
-          const uint16_t* src = p.y + (int64_t)max(t, 0) * p.ldy;
-          yv[b] = VEC ? load16(src + min(c + 8 * b, p.C - 8)) : load_some(src + c + 8 * b, min(8, p.C - c - 8 * b));
-        }
-      }
-      f32x4_t acc[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      wave_whole();
-#pragma unroll
-      for (int k = 0; k < KF; ++k) {
-        const u32x4_t hv = *(const u32x4_t*)&hs[k][16 * i + i16][8 * q];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = mfma_16x16x32<F16>(wv[k][j], hv, acc[j]);
-      }
-      if (t >= 0) {
-        uint16_t* dst = p.out + (int64_t)t * p.ldo + c;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          u32x4_t o;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            // columns 8 b + 2 e and the next one: fragment 2 b + e / 2, results 2 (e % 2) and the next one
-            const float v0 = f32_of_16<F16>((uint16_t)(yv[b][e] & 0xFFFFu)), v1 = f32_of_16<F16>((uint16_t)(yv[b][e] >> 16));
-            const f32x4_t& a = acc[2 * b + (e >> 1)];
-            o[e] = none ? yv[b][e] : pack_16x2<F16>(v0 + up * a[2 * (e & 1)], v1 + up * a[2 * (e & 1) + 1]);
-          }
-          const int n = min(8, p.C - c - 8 * b);
-          if (VEC) {
-            if (n > 0) *(u32x4_t*)(dst + 8 * b) = o;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e < n) dst[8 * b + e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
-          }
-        }
-      }
-      wave_whole();
-    }
+  int c0 = (int)c_begin + 64 * wave_id();
+  int t[MF];
+  lane_rows<MF>(p.rows, s, t);
+  Strip<F16, KF, MF, WT> strip;
+  if (c0 < c_end) strip.load(p, s.group, none, t, c0);  // under way while h is put together
+  put_h<F16, KF, MF, 256>(p, s, none, p.h && block == 0, p.part + (int64_t)s.padded * p.Rp, p.splits, (int64_t)p.P * p.Rp, p.Rp, hs, row_up);
+  __syncthreads();
+  if (none && p.out == p.y) return;
+  for (; c0 < c_end; c0 += 256) {
+    if (c0 >= c_begin + 256) strip.load(p, s.group, none, t, c0);
+    if (WT) strip.transpose(&tiles[WT ? wave_id() : 0][0][0]);
+    strip.finish(p, none, t, c0, hs, row_up);
   }
 }
 
-// ---- backward: transposed copies ----------------------------------------------------------------------------------------
-// dst[g][c][r] (rows of ldd) = src[g][r][c], for adapters that have rows. Elements between c < Cd's R and ldd are zeros.
-__global__ __launch_bounds__(256) void lora_transpose(const uint16_t* src, int Rs, int Cs, uint16_t* dst, int64_t ldd, Rows rows) {
-  __shared__ uint16_t tile[64][66];
-  const int g = blockIdx.z;
-  if (clamp_off(rows, g + 1) <= clamp_off(rows, g)) return;
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  const uint16_t* s = src + (int64_t)g * Rs * Cs;
-  for (int n = threadIdx.x; n < 64 * 64; n += 256) {
-    const int r = r0 + (n >> 6), c = c0 + (n & 63);
-    tile[n >> 6][n & 63] = r < Rs && c < Cs ? s[(int64_t)r * Cs + c] : (uint16_t)0;
+// ---- shrink and expand in one, for a few rows ---------------------------------------------------------------------------
+// Every workgroup of 16 rows and `cols` columns computes its rows' h again: that costs K R / 16 waves of loads from L2, which
+// is less than a second launch and a round trip through memory as long as A is small (see one_kernel).
+template <bool F16, int NF>
+__global__ __launch_bounds__(1024) void lora_few(ShrinkParams f, ExpandParams p, int slots) {
+  __shared__ __align__(16) uint16_t hs[NF][16][32];
+  __shared__ float row_up[16];
+  __shared__ __align__(16) float parts[16][16][16 * NF];
+  const int block = blockIdx.x / slots;
+  const Slot s = find_slot(p.rows, blockIdx.x - block * slots, 16);
+  if (s.group < 0) return;
+  const int lane = lane_id(), wave = wave_id(), i16 = lane & 15, q = lane >> 4;
+  const bool none = s.group == p.rows.G - 1;
+  const int c0 = block * p.cols + 64 * wave;
+  const bool mine = 64 * wave < p.cols && c0 < p.C;
+  int t[1];
+  lane_rows<1>(p.rows, s, t);
+  Strip<F16, NF, 1, false> strip;
+  if (mine) strip.load(p, s.group, none, t, c0);
+  if (!none) {
+    const uint16_t* xr[1];
+    const uint16_t* wr[NF];
+    shrink_rows<1>(p.rows, s, f.x, f.ldx, xr);
+    shrink_weights<NF>(s, f.w, f.ldw, f.R, wr);
+    f32x4_t acc[1][NF];
+#pragma unroll
+    for (int j = 0; j < NF; ++j) acc[0][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const int64_t begin = (int64_t)wave * f.per_wave;
+    shrink_columns<F16, NF, 1, (NF == 1 ? 4 : 2)>(xr, wr, (int)min(begin, (int64_t)f.C), (int)min((int64_t)f.C, begin + f.per_wave), q, acc);
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = 4 * q + e, r = 16 * j + i16;
+        parts[wave][n][r] = n < s.rows && r < f.R ? acc[0][j][e] : 0.f;
+      }
   }
   __syncthreads();
-  uint16_t* d = dst + (int64_t)g * Cs * ldd;
-  for (int n = threadIdx.x; n < 64 * 64; n += 256) {
-    const int c = c0 + (n >> 6), r = r0 + (n & 63);
-    if (c < Cs && r < ldd) d[(int64_t)c * ldd + r] = tile[n & 63][n >> 6];
-  }
+  put_h<F16, NF, 1, 1024>(p, s, none, p.h && block == 0, &parts[0][0][0], 16, 16 * 16 * NF, 16 * NF, hs, row_up);
+  __syncthreads();
+  if (mine && !(none && p.out == p.y)) strip.finish(p, none, t, c0, hs, row_up);
 }
 
 // ---- backward: the [rows, R] operand of wgrad ---------------------------------------------------------------------------
 // From the splits' parts (or from h as the forward pass returned it, in row order): for rank r and padded row n
-// hi[r][n], lo[r][n] = the two 16-bit parts of s_g * value, for fp16 times the power of two that suits the largest of the
-// chunk's rows; up[chunk slot][r] is its inverse. A workgroup takes one chunk and four ranks.
+// hi[r][n], lo[r][n] = the two 16-bit parts of s_g * value, for fp16 times the power of two that suits the largest of 32 rows
+// (one step of wgrad); up[padded row / 16][r] is its inverse, for the first of the 32 rows. sum (may be null) is the sum of the parts for expand.
 struct SmallParams {
   const float* part;
   const float* h;  // instead of part, [T, R]
   const float* scales;
   Rows rows;
-  int R, Rp, P, splits, chunk;
+  int R, Rp, P, splits;
   uint16_t* hi;  // [Rp][P]
   uint16_t* lo;
-  float* up;     // [chunk slots][Rp]
+  float* up;     // [P / 16][Rp]
+  float* sum;    // [P][Rp]
 };
 
-DEVINL float small_value(const SmallParams& p, const Slot& s, int n, int r, float scale) {
-  if (n >= s.rows || r >= p.R) return 0.f;
-  float v = 0.f;
-  if (p.h) {
-    const int t = p.rows.perm[s.first + n];
-    if (t >= 0 && t < p.rows.T) v = p.h[(int64_t)t * p.R + r];
-  } else {
-    for (int c = 0; c < p.splits; ++c) v += p.part[((int64_t)c * p.P + s.padded + n) * p.Rp + r];
-  }
-  return v * scale;
-}
-
+// A workgroup takes 32 rows. A thread takes four ranks of one of them; the 32 threads of a rank are neighbours. The parts are
+// dealt to as many strands of threads as there are threads for, whose sums meet in LDS.
 template <bool F16>
-__global__ __launch_bounds__(256) void lora_small(SmallParams p0, SmallParams p1) {
-  __shared__ float wave_max[4][4];
-  const SmallParams p = blockIdx.z ? p1 : p0;
-  const Slot s = find_slot(p.rows, blockIdx.x, p.chunk);
+__global__ __launch_bounds__(1024) void lora_small(SmallParams p) {
+  __shared__ f32x4_t strands[1024];
+  const Slot s = find_slot(p.rows, blockIdx.x, 32);
   if (s.group < 0 || s.group == p.rows.G - 1) return;
-  const int tid = threadIdx.x, r = blockIdx.y * 4 + (tid & 3);
+  const int n = threadIdx.x & 31, quads = p.Rp / 4, quad = (threadIdx.x >> 5) % quads, strand = (threadIdx.x >> 5) / quads;
+  const int many = 32 / quads, r = 4 * quad;  // Rp <= 128: at least one strand
   const float scale = p.scales ? p.scales[s.group] : 1.f;
-  float f = 1.f;
-  if (F16) {
-    float m = 0.f;
-    for (int n = tid >> 2; n < s.rows; n += 64) m = finite_max(m, small_value(p, s, n, r, scale));
-    wave_whole();
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  if (p.h) {
+    const int t = strand == 0 && n < s.rows ? p.rows.perm[s.first + n] : -1;
+    if (t >= 0 && t < p.rows.T)
 #pragma unroll
-    for (int d = 4; d < 64; d <<= 1) m = max(m, __shfl_xor(m, d, 64));
-    if (lane_id() < 4) wave_max[wave_id()][lane_id()] = m;
-    __syncthreads();
-    m = max(max(wave_max[0][tid & 3], wave_max[1][tid & 3]), max(wave_max[2][tid & 3], wave_max[3][tid & 3]));
-    f = pow2_down(m);
-    if (tid < 4) p.up[(int64_t)blockIdx.x * p.Rp + r] = pow2_up(m);
+      for (int e = 0; e < 4; ++e)
+        if (r + e < p.R) v[e] = p.h[(int64_t)t * p.R + r + e];
+  } else if (strand < many && n < s.rows) {
+    const int64_t next = (int64_t)p.P * p.Rp;
+    v = sum_parts<8>(p.part + (int64_t)(s.padded + n) * p.Rp + r + strand * next, p.splits - strand, many, next);
   }
-  for (int n = tid >> 2; n < ((s.rows + 15) & ~15); n += 64) {
-    uint16_t hi, lo;
-    split16<F16>(small_value(p, s, n, r, scale) * f, hi, lo);
-    p.hi[(int64_t)r * p.P + s.padded + n] = hi;
-    p.lo[(int64_t)r * p.P + s.padded + n] = lo;
+  strands[threadIdx.x] = v;
+  __syncthreads();
+  if (strand > 0) return;
+  for (int i = 1; i < many; ++i) v += strands[threadIdx.x + 32 * quads * i];
+  if (p.sum && n < s.rows) *(f32x4_t*)(p.sum + (int64_t)(s.padded + n) * p.Rp + r) = v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float a = v[e] * scale;
+    if (F16) {
+      float m = finite_max(0.f, a);
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) m = max(m, __shfl_xor(m, d, 64));
+      a *= pow2_down(m);
+      if (n == 0) p.up[(int64_t)(s.padded / 16) * p.Rp + r + e] = pow2_up(m);
+    }
+    if (n < ((s.rows + 15) & ~15)) {
+      uint16_t hi, lo;
+      split16<F16>(a, hi, lo);
+      p.hi[(int64_t)(r + e) * p.P + s.padded + n] = hi;
+      p.lo[(int64_t)(r + e) * p.P + s.padded + n] = lo;
+    }
   }
 }
 
 // ---- backward: wgrad ----------------------------------------------------------------------------------------------------
-// grad[c, r] = sum over the rows of an adapter of big[row, c] * small[row, r]. A workgroup takes up to `chunk` rows and 256
-// columns, 64 to a wave, in steps of 32 rows: the rows go through LDS as they are and are read back transposed
-// (ds_read_b64_tr_b16: four rows of 16 columns per 16 lanes), the small operand is laid out for the matrix instruction already.
+// grad[c, r] = sum over the rows of an adapter of big[row, c] * small[row, r]. A workgroup takes up to `chunk` rows, 256
+// columns (64 to a wave) and up to 64 ranks, in steps of 32 rows: the rows go through LDS as they are and are read back
+// transposed, the small operand is laid out for the matrix instruction already.
 // An adapter of one chunk is finished here; the sums of several are added in their order by lora_grad_sum, which also clears
 // the gradients of adapters without rows.
-struct GradJob {
+// OUT: big is the output's gradient, grad is gB as [C, R], and the same rows give the columns' share of u = gout B, part u[block]:
+// wave w multiplies rows 16 (w % 2) .. of a step with columns 128 (w / 2) .., whose B it keeps in registers as operands, and
+// the two halves of the columns meet in LDS one step later. Not OUT: big is x, grad is gA as [R, C].
+struct GradParams {
   const uint16_t* big;
   int64_t ld;
   const uint16_t* hi;
   const uint16_t* lo;
   const float* up;
-  uint16_t* grad;  // CR: [L, C, R], else [L, R, C]
-  float* part;     // [entries][C * R]
-  int C, vec, blocks;
-};
-struct GradParams {
-  GradJob job[2];  // gB (as [C, R]), gA (as [R, C])
+  uint16_t* grad;      // [L, C, R] or [L, R, C]
+  float* part;         // [entries][C * R]
+  const uint16_t* b;   // OUT: [L, C, R]
+  float* u;            // OUT: [blocks][P][Rp]
   Rows rows;
-  int R, Rp, P, chunk, slots, vec_store;  // vec_store: four neighbours of a gradient can be stored together
+  int C, R, Rp, P, chunk, slots, blocks;
 };
 
 constexpr int GRAD_ROW = 272;   // elements from row to row in LDS (256 columns and 32 bytes to spread the banks)
@@ -455,94 +628,176 @@ constexpr int GRAD_SKEW = 64;   // and after every eight rows
 DEVINL int grad_off(int row) { return row * GRAD_ROW + (row >> 3) * GRAD_SKEW; }
 constexpr int GRAD_TILE = 32 * GRAD_ROW + 4 * GRAD_SKEW;
 
-DEVINL u32x4_t read_transposed(const uint16_t* at) {
-  typedef __attribute__((address_space(3))) i16x4_t* lds_ptr;
-  const uint32_t a = (uint32_t)(uintptr_t)at;
-  const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(uintptr_t)a);
-  const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(uintptr_t)(a + 4 * GRAD_ROW * 2));
-  const u32x2_t l2 = __builtin_bit_cast(u32x2_t, lo), h2 = __builtin_bit_cast(u32x2_t, hi);
-  return u32x4_t{l2[0], l2[1], h2[0], h2[1]};
-}
-
-template <bool F16, int RF, bool CR>
-DEVINL void grad_body(const GradParams& p, const GradJob& job, int block, int slot, uint16_t* tile, uint16_t* small) {
+template <bool F16, int RF, bool OUT>
+__global__ __launch_bounds__(256) void lora_grad(GradParams p) {
+  constexpr int SMALL = 2 * RF * 16 * 4;        // 16-byte pieces of the small operand per step
+  constexpr int SL = (SMALL + 255) / 256;
+  __shared__ __align__(16) uint16_t tile[2][GRAD_TILE];
+  __shared__ __align__(16) uint16_t small[2][SMALL * 8];
+  __shared__ f32x4_t half_u[OUT ? 2 : 1][OUT ? 2 * RF : 1][64];
+  const int slot = blockIdx.x % p.slots, block = blockIdx.x / p.slots % p.blocks, r0 = blockIdx.x / p.slots / p.blocks * 16 * RF;
   const Slot s = find_slot(p.rows, slot, p.chunk);
   if (s.group < 0 || s.group == p.rows.G - 1) return;
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), i16 = lane & 15, q = lane >> 4;
   const int c0 = block * 256, rows16 = (s.rows + 15) & ~15;
-  f32x4_t acc[4][RF];
+  const int cl = c0 + 8 * (tid & 31), some = p.C - cl;  // this thread's eight columns of the rows tid / 32 + 8 j
+
+  // B of this wave's 128 columns, ranks r0 ..: through the tile, one half of the columns after the other
+  u32x4_t bt[OUT ? 4 : 1][RF];
+  if (OUT) {
+    constexpr int ROW = RF * 16 + 8;
+    static_assert(128 * ROW <= 2 * GRAD_TILE, "128 columns of B fit the tiles");
+    uint16_t* at = tile[0];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      for (int n = tid; n < 128 * RF * 2; n += 256) {
+        const int c = c0 + 128 * half + n / (RF * 2), r = r0 + 8 * (n % (RF * 2));
+        u32x4_t v = {0u, 0u, 0u, 0u};
+        if (c < p.C) {
+          const uint16_t* src = p.b + ((int64_t)s.group * p.C + c) * p.R + r;
+          if (r + 8 <= p.R) v = load16(src);
+          else if (r < p.R) v = load_some(src, p.R - r);
+        }
+        *(u32x4_t*)(at + (n / (RF * 2)) * ROW + 8 * (n % (RF * 2))) = v;
+      }
+      __syncthreads();
+      if ((wave >> 1) == half)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int f = 0; f < RF; ++f) bt[k][f] = read_transposed(at + (32 * k + 8 * q + (i16 >> 2)) * ROW + 16 * f + 4 * (i16 & 3), 4 * ROW * 2);
+      __syncthreads();
+    }
+  }
+
+  f32x4_t acc[4][RF], au[RF];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int f = 0; f < RF; ++f) acc[j][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  constexpr int SMALL = 2 * RF * 16 * 4;        // 16-byte pieces of the small operand per step
-  constexpr int SL = (SMALL + 255) / 256;
-  u32x4_t bv[4], sv[SL];
-  auto load = [&](int n0) {
+  auto row_of = [&](int n, int (&t)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int n = n0 + (tid >> 5) + 8 * j, c = c0 + 8 * (tid & 31);
-      const int t = n < s.rows ? p.rows.perm[s.first + n] : -1;
-      const int some = t >= 0 && t < p.rows.T ? min(8, job.C - c) : 0;
+      t[j] = n + (tid >> 5) + 8 * j < s.rows ? p.rows.perm[s.first + n + (tid >> 5) + 8 * j] : -1;
+      if (t[j] >= p.rows.T) t[j] = -1;
+    }
+  };
+  u32x4_t bv[4], sv[SL];
+  const bool edge = c0 + 256 > p.C;
+  auto load = [&](int n0, const int (&t)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
       bv[j] = u32x4_t{0u, 0u, 0u, 0u};
-      if (some > 0) {
-        const uint16_t* src = job.big + (int64_t)t * job.ld + c;
-        bv[j] = job.vec ? load16(src) : load_some(src, some);
-      }
+      const uint16_t* src = p.big + (int64_t)max(t[j], 0) * p.ld + cl;
+      if (!edge) bv[j] = t[j] >= 0 ? load16(src) : bv[j];
+      else if (t[j] >= 0) bv[j] = some >= 8 ? load16(src) : load_some(src, some);
     }
 #pragma unroll
     for (int j = 0; j < SL; ++j) {
-      const int i = tid + 256 * j, n = n0 + 8 * (i & 3), r = (i >> 2) % (RF * 16);
+      const int i = tid + 256 * j, n = n0 + 8 * (i & 3), r = r0 + (i >> 2) % (RF * 16);
       sv[j] = u32x4_t{0u, 0u, 0u, 0u};
-      if (i < SMALL && n < rows16 && r < p.Rp) sv[j] = load16((i >= SMALL / 2 ? job.lo : job.hi) + (int64_t)r * p.P + s.padded + n);
+      if (i < SMALL && n < rows16 && r < p.Rp) sv[j] = load16((i >= SMALL / 2 ? p.lo : p.hi) + (int64_t)r * p.P + s.padded + n);
     }
   };
-  load(0);
+  // this wave's share of u for the rows of the step before, waves 0 and 1: with the other half's
+  auto write_u = [&](int n0) {
+    const int n = n0 + 16 * wave;
+    if (wave < 2 && n < rows16) {
+      float* u = p.u + ((int64_t)block * p.P + s.padded + n) * p.Rp + r0;
+#pragma unroll
+      for (int f = 0; f < RF; ++f) {
+        const f32x4_t v = au[f] + half_u[(n0 >> 5) & 1][wave * RF + f][lane];
+        if (r0 + 16 * f < p.Rp)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[(int64_t)(4 * q + e) * p.Rp + 16 * f + i16] = v[e];
+      }
+    }
+  };
+  int t[4];
+  row_of(0, t);
+  load(0, t);
+  row_of(32, t);
   int buf = 0;
   for (int n0 = 0; n0 < s.rows; n0 += 32, buf ^= 1) {
-    uint16_t* tl = tile + buf * GRAD_TILE;
-    uint16_t* sm = small + buf * (SMALL * 8);
+    uint16_t* tl = tile[buf];
+    uint16_t* sm = small[buf];
 #pragma unroll
     for (int j = 0; j < 4; ++j) *(u32x4_t*)(tl + grad_off((tid >> 5) + 8 * j) + 8 * (tid & 31)) = bv[j];
 #pragma unroll
     for (int j = 0; j < SL; ++j)
       if (tid + 256 * j < SMALL) *(u32x4_t*)(sm + (tid + 256 * j) * 8) = sv[j];
-    if (n0 + 32 < s.rows) load(n0 + 32);
+    if (n0 + 32 < s.rows) {
+      load(n0 + 32, t);
+      row_of(n0 + 64, t);
+    }
     __syncthreads();
+    if (OUT) {
+      if (n0 > 0) write_u(n0 - 32);
+#pragma unroll
+      for (int f = 0; f < RF; ++f) au[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const u32x4_t v = *(const u32x4_t*)(tl + grad_off(16 * (wave & 1) + i16) + 128 * (wave >> 1) + 32 * k + 8 * q);
+#pragma unroll
+        for (int f = 0; f < RF; ++f) au[f] = mfma_16x16x32<F16>(v, bt[k][f], au[f]);
+      }
+      if (wave >= 2)
+#pragma unroll
+        for (int f = 0; f < RF; ++f) half_u[(n0 >> 5) & 1][(wave - 2) * RF + f][lane] = au[f];
+    }
     u32x4_t b[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) b[j] = read_transposed(tl + grad_off(8 * q + (i16 >> 2)) + 64 * wave + 16 * j + 4 * (i16 & 3));
+    for (int j = 0; j < 4; ++j)
+      b[j] = read_transposed(tl + grad_off(8 * q + (i16 >> 2)) + 64 * wave + 16 * j + 4 * (i16 & 3), 4 * GRAD_ROW * 2);
 #pragma unroll
-    for (int f = 0; f < RF; ++f)
+    for (int f = 0; f < RF; ++f) {
+      u32x4_t v[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const u32x4_t v = *(const u32x4_t*)(sm + ((h * RF * 16 + 16 * f + i16) * 4 + q) * 8);
+      for (int h = 0; h < 2; ++h) v[h] = *(const u32x4_t*)(sm + ((h * RF * 16 + 16 * f + i16) * 4 + q) * 8);
+      if (F16) {
+        // a step has its own scale for each rank: its products are summed apart and scaled back
+        const int r = r0 + 16 * f + (OUT ? 4 * q : i16);
+        const float* up = p.up + (int64_t)((s.padded + n0) / 16) * p.Rp;
+        f32x4_t scale;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j][f] = CR ? mfma_16x16x32<F16>(v, b[j], acc[j][f]) : mfma_16x16x32<F16>(b[j], v, acc[j][f]);
+        for (int e = 0; e < 4; ++e) scale[e] = r + (OUT ? e : 0) < p.Rp ? up[r + (OUT ? e : 0)] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) d = OUT ? mfma_16x16x32<F16>(v[h], b[j], d) : mfma_16x16x32<F16>(b[j], v[h], d);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][f][e] += d[e] * scale[e];
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j][f] = OUT ? mfma_16x16x32<F16>(v[h], b[j], acc[j][f]) : mfma_16x16x32<F16>(b[j], v[h], acc[j][f]);
       }
+    }
+  }
+  if (OUT) {
+    __syncthreads();
+    write_u((s.rows - 1) & ~31);
   }
   const bool whole = s.size <= p.chunk;
-  const int64_t block_size = (int64_t)job.C * p.R;
+  const int64_t block_size = (int64_t)p.C * p.R;
   const int64_t entry = s.begin / (p.chunk / 2) + (s.first - s.begin) / p.chunk;
-  uint16_t* grad = job.grad + s.group * block_size;
-  float* part = job.part + entry * block_size;
+  uint16_t* grad = p.grad + s.group * block_size;
+  float* part = p.part + entry * block_size;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int f = 0; f < RF; ++f) {
-      const int c = c0 + 64 * wave + 16 * j + (CR ? i16 : 4 * q), r = 16 * f + (CR ? 4 * q : i16);
-      if (c >= job.C || r >= p.R) continue;
-      f32x4_t v = acc[j][f];
-      if (F16) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= job.up[(int64_t)slot * p.Rp + r + (CR ? e : 0)];
-      }
-      const int64_t at = CR ? (int64_t)c * p.R + r : (int64_t)r * job.C + c;
-      const int n = min(4, CR ? p.R - r : job.C - c);
-      if (p.vec_store) {
-        if (whole) *(u32x2_t*)(grad + at) = u32x2_t{pack_16x2<F16>(v[0], v[1]), pack_16x2<F16>(v[2], v[3])};
-        else *(f32x4_t*)(part + at) = v;
+      const int c = c0 + 64 * wave + 16 * j + (OUT ? i16 : 4 * q), r = r0 + 16 * f + (OUT ? 4 * q : i16);
+      if (c >= p.C || r >= p.R) continue;
+      const f32x4_t v = acc[j][f];
+      const int64_t at = OUT ? (int64_t)c * p.R + r : (int64_t)r * p.C + c;
+      const int n = min(4, OUT ? p.R - r : p.C - c);
+      if (n == 4) {
+        if (whole) *(u32x2_any_t*)(grad + at) = u32x2_t{pack_16x2<F16>(v[0], v[1]), pack_16x2<F16>(v[2], v[3])};
+        else *(f32x4_any_t*)(part + at) = v;
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -554,108 +809,123 @@ DEVINL void grad_body(const GradParams& p, const GradJob& job, int block, int sl
     }
 }
 
-template <bool F16, int RF>
-__global__ __launch_bounds__(256) void lora_grad(GradParams p) {
-  __shared__ __align__(16) uint16_t tile[2 * GRAD_TILE];
-  __shared__ __align__(16) uint16_t small[2 * 2 * RF * 16 * 32];
-  const int slot = blockIdx.x % p.slots, block = blockIdx.x / p.slots;
-  if (block < p.job[0].blocks) grad_body<F16, RF, true>(p, p.job[0], block, slot, tile, small);
-  else grad_body<F16, RF, false>(p, p.job[1], block - p.job[0].blocks, slot, tile, small);
+// The gradients of adapters of several chunks, of both jobs; a thread takes eight elements.
+template <bool F16>
+__global__ __launch_bounds__(256) void lora_grad_sum(GradParams p0, GradParams p1, int blocks0) {
+  const int g = blockIdx.y;
+  const bool first = (int)blockIdx.x < blocks0;
+  const Rows rows = p0.rows;
+  const int chunk = first ? p0.chunk : p1.chunk, C = first ? p0.C : p1.C;
+  const int begin = clamp_off(rows, g), size = clamp_off(rows, g + 1) - begin;
+  if (size > 0 && size <= chunk) return;
+  const int64_t block_size = (int64_t)C * p0.R;
+  const int64_t i = ((int64_t)(blockIdx.x - (first ? 0 : blocks0)) * 256 + threadIdx.x) * 8;
+  if (i >= block_size) return;
+  const int n = (int)min((int64_t)8, block_size - i);
+  const int chunks = size > 0 ? (size + chunk - 1) / chunk : 0;
+  const float* part = (first ? p0.part : p1.part) + (int64_t)(begin / (chunk / 2)) * block_size + i;
+  uint16_t* d = (first ? p0.grad : p1.grad) + g * block_size + i;
+  if (n == 8) {
+    f32x4_t v[2] = {};
+    for (int c = 0; c < chunks; ++c, part += block_size) {
+      v[0] += *(const f32x4_any_t*)part;
+      v[1] += *(const f32x4_any_t*)(part + 4);
+    }
+    store16(d, u32x4_t{pack_16x2<F16>(v[0][0], v[0][1]), pack_16x2<F16>(v[0][2], v[0][3]), pack_16x2<F16>(v[1][0], v[1][1]), pack_16x2<F16>(v[1][2], v[1][3])});
+    return;
+  }
+  for (int e = 0; e < n; ++e) {
+    float v = 0.f;
+    for (int c = 0; c < chunks; ++c) v += part[c * block_size + e];
+    d[e] = cvt_16<F16>(v);
+  }
 }
 
-template <bool F16>
-__global__ __launch_bounds__(256) void lora_grad_sum(GradParams p, int blocks0) {
-  const int g = blockIdx.y;
-  const int begin = clamp_off(p.rows, g), size = clamp_off(p.rows, g + 1) - begin;
-  if (size > 0 && size <= p.chunk) return;
-  const bool first = (int)blockIdx.x < blocks0;
-  const GradJob& job = first ? p.job[0] : p.job[1];
-  const int64_t block_size = (int64_t)job.C * p.R;
-  const int64_t i = ((int64_t)(blockIdx.x - (first ? 0 : blocks0)) * 256 + threadIdx.x) * 4;
-  if (i >= block_size) return;
-  const int n = (int)min((int64_t)4, block_size - i);
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
-  const int chunks = size > 0 ? (size + p.chunk - 1) / p.chunk : 0;
-  for (int c = 0; c < chunks; ++c) {
-    const float* part = job.part + ((int64_t)(begin / (p.chunk / 2)) + c) * block_size + i;
-    for (int e = 0; e < n; ++e) v[e] += part[e];
-  }
-  uint16_t* d = job.grad + g * block_size + i;
-  for (int e = 0; e < n; ++e) d[e] = cvt_16<F16>(v[e]);
-}
+int slots_of(int64_t T, int64_t G, int unit) { return (int)(T == 0 ? 1 : T < T / unit + G ? T : T / unit + G); }
 
 template <bool F16, int NF, int MF>
-void launch_shrink(const ShrinkParams& p, bool vec, hipStream_t stream) {
-  const int slots = p.rows.T / (16 * MF) + p.rows.G;
-  const dim3 grid(slots * p.splits), block(512);
-  if (vec) hipLaunchKernelGGL((lora_shrink<F16, NF, MF, true>), grid, block, 0, stream, p, slots);
-  else hipLaunchKernelGGL((lora_shrink<F16, NF, MF, false>), grid, block, 0, stream, p, slots);
+void launch_shrink(const ShrinkParams& p, hipStream_t stream) {
+  const int slots = slots_of(p.rows.T, p.rows.G, 16 * MF);
+  hipLaunchKernelGGL((lora_shrink<F16, NF, MF>), dim3(slots * p.splits), dim3(512), 0, stream, p, slots);
 }
 
-template <bool F16, int KF, int MF>
-void launch_expand(const ExpandParams& p, bool vec, hipStream_t stream) {
-  const int slots = p.rows.T / (16 * MF) + p.rows.G;
-  const dim3 grid(slots * ((p.C + p.cols - 1) / p.cols)), block(256);
-  if (vec) hipLaunchKernelGGL((lora_expand<F16, KF, MF, true>), grid, block, 0, stream, p, slots);
-  else hipLaunchKernelGGL((lora_expand<F16, KF, MF, false>), grid, block, 0, stream, p, slots);
+template <bool F16, int KF, int MF, bool WT>
+void launch_expand(const ExpandParams& p, hipStream_t stream) {
+  const int slots = slots_of(p.rows.T, p.rows.G, 16 * MF);
+  hipLaunchKernelGGL((lora_expand<F16, KF, MF, WT>), dim3(slots * ((p.C + p.cols - 1) / p.cols)), dim3(256), 0, stream, p, slots);
 }
 
-bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 int rank_blocks(int R) { return R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8; }
-// Rows per workgroup of shrink and expand: 64 (32 for the highest ranks in shrink) reuse an adapter's weights over more
-// rows, 16 give more workgroups; below 512 rows there are too few of the former to fill the card.
-constexpr int MANY_ROWS = 512;
+int64_t tiles_of(int64_t T, int64_t G, int rows) { return T / rows + (G < T ? G : T); }
+// Rows per workgroup of shrink and expand: 64 (32 for the highest ranks) use an adapter's weights for more rows, 16 give more
+// workgroups. 64 once those, with 256 of the C columns each, fill the card.
+int rows_of(int64_t T, int R, int C) {
+  const int many = rank_blocks(R) == 8 ? 32 : 64;
+  return T / many * ((C + 255) / 256) >= 256 ? many : 16;
+}
 
 template <bool F16>
 void shrink(const ShrinkParams& p, hipStream_t stream) {
-  const bool vec = p.C % 8 == 0 && p.ldx % 8 == 0 && p.ldw % 8 == 0 && aligned16(p.x) && aligned16(p.w);
-  const bool many = p.rows.T >= MANY_ROWS;
+  const bool many = rows_of(p.rows.T, p.R, p.C) > 16;
   switch (rank_blocks(p.R)) {
-    case 1: many ? launch_shrink<F16, 1, 4>(p, vec, stream) : launch_shrink<F16, 1, 1>(p, vec, stream); break;
-    case 2: many ? launch_shrink<F16, 2, 4>(p, vec, stream) : launch_shrink<F16, 2, 1>(p, vec, stream); break;
-    case 4: many ? launch_shrink<F16, 4, 4>(p, vec, stream) : launch_shrink<F16, 4, 1>(p, vec, stream); break;
-    default: many ? launch_shrink<F16, 8, 2>(p, vec, stream) : launch_shrink<F16, 8, 1>(p, vec, stream); break;
+    case 1: many ? launch_shrink<F16, 1, 4>(p, stream) : launch_shrink<F16, 1, 1>(p, stream); break;
+    case 2: many ? launch_shrink<F16, 2, 4>(p, stream) : launch_shrink<F16, 2, 1>(p, stream); break;
+    case 4: many ? launch_shrink<F16, 4, 4>(p, stream) : launch_shrink<F16, 4, 1>(p, stream); break;
+    default: many ? launch_shrink<F16, 8, 2>(p, stream) : launch_shrink<F16, 8, 1>(p, stream); break;
   }
 }
 
-template <bool F16>
-void expand(const ExpandParams& p, hipStream_t stream) {
-  const bool vec = p.C % 8 == 0 && p.ldy % 8 == 0 && p.ldo % 8 == 0 && aligned16(p.y) && aligned16(p.out);
-  const bool many = p.rows.T >= MANY_ROWS;
+// Columns per workgroup of expand: 1024 (four strips per wave) once that fills the card, else 256.
+template <bool F16, bool WT>
+void expand(ExpandParams p, hipStream_t stream) {
+  const int rows = rows_of(p.rows.T, p.R, p.C);
+  const bool many = rows > 16;
+  p.cols = tiles_of(p.rows.T, p.rows.G, rows) * ((p.C + 1023) / 1024) >= 512 ? 1024 : 256;
   switch (rank_blocks(p.R)) {
-    case 1: many ? launch_expand<F16, 1, 4>(p, vec, stream) : launch_expand<F16, 1, 1>(p, vec, stream); break;
-    case 2: many ? launch_expand<F16, 2, 4>(p, vec, stream) : launch_expand<F16, 2, 1>(p, vec, stream); break;
-    case 4: many ? launch_expand<F16, 4, 4>(p, vec, stream) : launch_expand<F16, 4, 1>(p, vec, stream); break;
-    default: many ? launch_expand<F16, 8, 4>(p, vec, stream) : launch_expand<F16, 8, 1>(p, vec, stream); break;
+    case 1: many ? launch_expand<F16, 1, 4, WT>(p, stream) : launch_expand<F16, 1, 1, WT>(p, stream); break;
+    case 2: many ? launch_expand<F16, 2, 4, WT>(p, stream) : launch_expand<F16, 2, 1, WT>(p, stream); break;
+    case 4: many ? launch_expand<F16, 4, 4, WT>(p, stream) : launch_expand<F16, 4, 1, WT>(p, stream); break;
+    default: many ? launch_expand<F16, 8, 2, WT>(p, stream) : launch_expand<F16, 8, 1, WT>(p, stream); break;
   }
 }
 
-// Splits of the reduced axis: until about 512 workgroups (two to a CU), but 64 columns at least for each of the eight waves
-// and at most 16 parts, which the next kernel adds again for every row.
-int shrink_splits(int64_t T, int G, int R, int C) {
-  const int64_t rows = T >= MANY_ROWS ? (rank_blocks(R) == 8 ? 32 : 64) : 16;
-  const int64_t tiles = T / rows + (G < T ? G : T) + (T == 0);
-  const int64_t most = (C + 511) / 512;
-  int64_t s = 512 / tiles;
+// Columns per wave of shrink, a multiple of 64: the reduced axis is split until there are about 1024 workgroups, into at most
+// 16 parts, which the next kernel adds again for every row.
+int shrink_per_wave(int64_t T, int64_t G, int R, int C) {
+  int64_t s = 1024 / (tiles_of(T, G, rows_of(T, R, C)) + 1);
   s = s < 1 ? 1 : s > 16 ? 16 : s;
-  return (int)(s < most ? s : most);
+  return (int)((C + 512 * s - 1) / (512 * s) * 64);
 }
-int per_wave(int C, int splits) { return (int)((((int64_t)C + 64 * 8 * splits - 1) / (64 * 8 * splits)) * 64); }
+int splits_of(int C, int per_wave) { return (C + 8 * per_wave - 1) / (8 * per_wave); }
+
+// Few rows, and an A that sixteen waves read in a few microseconds.
+bool one_kernel(int64_t T, int K, int R) { return T <= 128 && R <= 32 && (int64_t)K * rank_blocks(R) <= 8192; }
+
+// Rows of a workgroup of wgrad: 512, or half or a quarter of that until there are about 400 workgroups; with more rows than
+// 8192 more, so that the partial sums of an adapter of several chunks stay at 32 times its gradients.
+int grad_chunk(int64_t T, int C) {
+  if (T > 8192) return (int)(512 * ((T + 8191) / 8192));
+  int chunk = 512;
+  while (chunk > 128 && T / chunk * ((C + 255) / 256) < 384) chunk /= 2;
+  return chunk;
+}
+int64_t grad_entries(int64_t T, int chunk) { return T / (chunk / 2); }
 
 struct Sizes {
-  int64_t G, P, Rp, chunk, slots, entries;
-  int s_x, s_g;
+  int64_t G, P, Rp, blocks;
+  int chunk[2];  // rows of a workgroup of wgrad on the output's gradient and on x
+  int s_x, w_x;  // shrink of x: splits, columns per wave
 };
 Sizes sizes_of(int64_t T, int L, int K, int N, int R) {
   Sizes z;
   z.G = L + 1;
   z.P = 16 * (T / 16 + z.G);
   z.Rp = (R + 15) / 16 * 16;
-  z.chunk = 512 * (T > 8192 ? (T + 8191) / 8192 : 1);
-  z.slots = T / z.chunk + z.G;
-  z.entries = T / (z.chunk / 2);
-  z.s_x = shrink_splits(T, (int)z.G, R, K);
-  z.s_g = shrink_splits(T, (int)z.G, R, N);
+  z.blocks = (N + 255) / 256;
+  z.chunk[0] = grad_chunk(T, N);
+  z.chunk[1] = grad_chunk(T, K);
+  z.w_x = shrink_per_wave(T, z.G, R, K);
+  z.s_x = splits_of(K, z.w_x);
   return z;
 }
 
@@ -670,22 +940,21 @@ struct Workspace {
 };
 
 struct BackwardSpace {
-  uint16_t *bt, *at, *hi[2], *lo[2];
-  float *part_u, *part_h, *up[2], *sums[2];
+  uint16_t *hi[2], *lo[2];                               // 0: h, 1: u
+  float *part_u, *part_h, *sum_u, *up[2], *sums[2];
 };
-BackwardSpace backward_space(Workspace& w, const Sizes& z, int L, int K, int N, int R, bool with_h) {
+BackwardSpace backward_space(Workspace& w, const Sizes& z, int64_t T, int K, int N, int R, bool with_h) {
   BackwardSpace b;
-  b.bt = w.take<uint16_t>((int64_t)L * R * ((N + 7) / 8 * 8));
-  b.at = w.take<uint16_t>((int64_t)L * K * ((R + 7) / 8 * 8));
-  b.part_u = w.take<float>(z.s_g * z.P * z.Rp);
+  b.part_u = w.take<float>(z.blocks * z.P * z.Rp);
   b.part_h = with_h ? nullptr : w.take<float>(z.s_x * z.P * z.Rp);
+  b.sum_u = w.take<float>(z.P * z.Rp);
   for (int j = 0; j < 2; ++j) {
     b.hi[j] = w.take<uint16_t>(z.Rp * z.P);
     b.lo[j] = w.take<uint16_t>(z.Rp * z.P);
-    b.up[j] = w.take<float>(z.slots * z.Rp);
+    b.up[j] = w.take<float>(z.P / 16 * z.Rp);
   }
-  b.sums[0] = w.take<float>(z.entries * N * R);
-  b.sums[1] = w.take<float>(z.entries * K * R);
+  b.sums[0] = w.take<float>(grad_entries(T, z.chunk[0]) * N * R);
+  b.sums[1] = w.take<float>(grad_entries(T, z.chunk[1]) * K * R);
   return b;
 }
 
@@ -695,98 +964,85 @@ __global__ __launch_bounds__(256) void lora_keys(const int32_t* ids, int32_t* ke
   if (t < T) keys[t] = ids[t] >= 0 && ids[t] < L ? ids[t] : L;
 }
 
-ShrinkParams shrink_params(const void* x, int64_t ldx, const void* w, int64_t ldw, float* part, const Rows& rows, int C, int R, const Sizes& z, int splits) {
-  ShrinkParams p{};
-  p.x = (const uint16_t*)x; p.ldx = ldx; p.w = (const uint16_t*)w; p.ldw = ldw; p.part = part; p.rows = rows;
-  p.C = C; p.R = R; p.Rp = (int)z.Rp; p.P = (int)z.P; p.splits = splits; p.per_wave = per_wave(C, splits);
-  return p;
-}
-
-// Columns per workgroup of expand: 1024 (four strips per wave) once that fills the card, else 256.
-int expand_cols(int64_t T, int G, int C) {
-  const int64_t rows = T >= MANY_ROWS ? 64 : 16;
-  const int64_t tiles = T / rows + (G < T ? G : T);
-  return tiles * ((C + 1023) / 1024) >= 512 ? 1024 : 256;
+ShrinkParams shrink_params(const LoraParams& p, const Rows& rows, const Sizes& z, float* part) {
+  ShrinkParams f{};
+  f.x = (const uint16_t*)p.x; f.ldx = p.ldx; f.w = (const uint16_t*)p.a; f.ldw = p.K; f.part = part; f.rows = rows;
+  f.C = p.K; f.R = p.R; f.Rp = (int)z.Rp; f.P = (int)z.P; f.per_wave = z.w_x; f.splits = z.s_x;
+  return f;
 }
 
 template <bool F16>
 void forward(const LoraParams& p, hipStream_t stream) {
   const Sizes z = sizes_of(p.T, p.L, p.K, p.N, p.R);
   const Rows rows{p.perm, p.offsets, (int)z.G, p.T};
-  float* part = (float*)p.workspace;
-  if (p.L > 0) shrink<F16>(shrink_params(p.x, p.ldx, p.a, p.K, part, rows, p.K, p.R, z, z.s_x), stream);
+  ShrinkParams f = shrink_params(p, rows, z, (float*)p.workspace);
   ExpandParams e{};
-  e.part = part; e.w = (const uint16_t*)p.b; e.ldw = p.R; e.wvec = p.R % 8 == 0 && aligned16(p.b); e.scales = p.scales;
-  e.y = (const uint16_t*)p.y; e.ldy = p.ldy; e.out = (uint16_t*)p.out; e.ldo = p.ldo; e.h = (float*)p.h; e.rows = rows;
-  e.C = p.N; e.R = p.R; e.Rp = (int)z.Rp; e.P = (int)z.P; e.splits = z.s_x; e.cols = expand_cols(p.T, (int)z.G, p.N);
-  expand<F16>(e, stream);
+  e.part = f.part; e.w = (const uint16_t*)p.b; e.scales = p.scales; e.y = (const uint16_t*)p.y; e.ldy = p.ldy; e.out = (uint16_t*)p.out;
+  e.ldo = p.ldo; e.h = (float*)p.h; e.rows = rows; e.C = p.N; e.R = p.R; e.Rp = (int)z.Rp; e.P = (int)z.P; e.splits = z.s_x;
+  if (one_kernel(p.T, p.K, p.R)) {
+    const int slots = slots_of(p.T, z.G, 16);
+    f.per_wave = (p.K + 1023) / 1024 * 64;
+    e.cols = 256;
+    while (e.cols < 1024 && tiles_of(p.T, z.G, 16) * ((p.N + e.cols - 1) / e.cols) > 512) e.cols *= 2;
+    const dim3 grid(slots * ((p.N + e.cols - 1) / e.cols)), block(1024);
+    if (p.R <= 16) hipLaunchKernelGGL((lora_few<F16, 1>), grid, block, 0, stream, f, e, slots);
+    else hipLaunchKernelGGL((lora_few<F16, 2>), grid, block, 0, stream, f, e, slots);
+    return;
+  }
+  if (p.L > 0) shrink<F16>(f, stream);
+  expand<F16, false>(e, stream);
 }
 
-template <bool F16, int RF>
+template <bool F16, bool OUT>
 void launch_grad(const GradParams& g, hipStream_t stream) {
-  hipLaunchKernelGGL((lora_grad<F16, RF>), dim3(g.slots * (g.job[0].blocks + g.job[1].blocks)), dim3(256), 0, stream, g);
+  const int rf = rank_blocks(g.R) > 4 ? 4 : rank_blocks(g.R);
+  const dim3 grid(g.slots * g.blocks * ((g.R + 16 * rf - 1) / (16 * rf))), block(256);
+  if (rf == 1) hipLaunchKernelGGL((lora_grad<F16, 1, OUT>), grid, block, 0, stream, g);
+  else if (rf == 2) hipLaunchKernelGGL((lora_grad<F16, 2, OUT>), grid, block, 0, stream, g);
+  else hipLaunchKernelGGL((lora_grad<F16, 4, OUT>), grid, block, 0, stream, g);
 }
 
 template <bool F16>
 void backward(const LoraParams& p, hipStream_t stream) {
   const Sizes z = sizes_of(p.T, p.L, p.K, p.N, p.R);
   Workspace w{(char*)p.workspace, 0};
-  const BackwardSpace b = backward_space(w, z, p.L, p.K, p.N, p.R, p.h != nullptr);
+  const BackwardSpace b = backward_space(w, z, p.T, p.K, p.N, p.R, p.h != nullptr);
   const Rows rows{p.perm, p.offsets, (int)z.G, p.T};
-  const int Nd = (p.N + 7) / 8 * 8, Rd = (p.R + 7) / 8 * 8;
   ExpandParams e{};
-  e.part = b.part_u; e.w = b.at; e.ldw = Rd; e.wvec = 1; e.scales = p.scales; e.y = (const uint16_t*)p.gx_in; e.ldy = p.ld_gx_in;
-  e.out = (uint16_t*)p.gx; e.ldo = p.ld_gx; e.rows = rows; e.C = p.K; e.R = p.R; e.Rp = (int)z.Rp; e.P = (int)z.P; e.splits = z.s_g;
-  e.cols = expand_cols(p.T, (int)z.G, p.K);
-  if (!e.y) e.ldy = e.ldo;
-  if (p.L == 0) return expand<F16>(e, stream);
-  hipLaunchKernelGGL(lora_transpose, dim3((p.R + 63) / 64, (Nd + 63) / 64, p.L), dim3(256), 0, stream, (const uint16_t*)p.b, p.N, p.R, b.bt, (int64_t)Nd, rows);
-  hipLaunchKernelGGL(lora_transpose, dim3((p.K + 63) / 64, (Rd + 63) / 64, p.L), dim3(256), 0, stream, (const uint16_t*)p.a, p.R, p.K, b.at, (int64_t)Rd, rows);
-  shrink<F16>(shrink_params(p.y, p.ldy, b.bt, Nd, b.part_u, rows, p.N, p.R, z, z.s_g), stream);
-  if (!p.h) shrink<F16>(shrink_params(p.x, p.ldx, p.a, p.K, b.part_h, rows, p.K, p.R, z, z.s_x), stream);
-  SmallParams sp[2] = {};
-  for (int j = 0; j < 2; ++j) {  // 0: h for gB, 1: u for gA
-    sp[j].part = j ? b.part_u : b.part_h;
-    sp[j].h = j ? nullptr : (const float*)p.h;
-    sp[j].scales = p.scales; sp[j].rows = rows; sp[j].R = p.R; sp[j].Rp = (int)z.Rp; sp[j].P = (int)z.P;
-    sp[j].splits = j ? z.s_g : z.s_x; sp[j].chunk = (int)z.chunk; sp[j].hi = b.hi[j]; sp[j].lo = b.lo[j]; sp[j].up = b.up[j];
+  e.part = b.sum_u; e.w = (const uint16_t*)p.a; e.scales = p.scales; e.y = (const uint16_t*)p.gx_in; e.ldy = p.gx_in ? p.ld_gx_in : p.ld_gx;
+  e.out = (uint16_t*)p.gx; e.ldo = p.ld_gx; e.rows = rows; e.C = p.K; e.R = p.R; e.Rp = (int)z.Rp; e.P = (int)z.P; e.splits = 1;
+  if (p.L == 0) return expand<F16, true>(e, stream);
+  if (!p.h) shrink<F16>(shrink_params(p, rows, z, b.part_h), stream);
+  GradParams g[2] = {};
+  for (int j = 0; j < 2; ++j) {  // 0: gB and u from the output's gradient and h; 1: gA from x and u
+    SmallParams sp{};
+    sp.part = j ? b.part_u : b.part_h; sp.h = j ? nullptr : (const float*)p.h; sp.scales = p.scales; sp.rows = rows;
+    sp.R = p.R; sp.Rp = (int)z.Rp; sp.P = (int)z.P; sp.splits = j ? (int)z.blocks : z.s_x;
+    sp.hi = b.hi[j]; sp.lo = b.lo[j]; sp.up = b.up[j]; sp.sum = j ? b.sum_u : nullptr;
+    hipLaunchKernelGGL((lora_small<F16>), dim3(slots_of(p.T, z.G, 32)), dim3(1024), 0, stream, sp);
+    g[j].big = (const uint16_t*)(j ? p.x : p.y); g[j].ld = j ? p.ldx : p.ldy;
+    g[j].hi = b.hi[j]; g[j].lo = b.lo[j]; g[j].up = b.up[j];
+    g[j].grad = (uint16_t*)(j ? p.grad_a : p.grad_b); g[j].part = b.sums[j]; g[j].b = (const uint16_t*)p.b; g[j].u = b.part_u;
+    g[j].rows = rows; g[j].C = j ? p.K : p.N; g[j].R = p.R; g[j].Rp = (int)z.Rp; g[j].P = (int)z.P;
+    g[j].chunk = z.chunk[j]; g[j].slots = slots_of(p.T, z.G, z.chunk[j]); g[j].blocks = (g[j].C + 255) / 256;
+    j ? launch_grad<F16, false>(g[j], stream) : launch_grad<F16, true>(g[j], stream);
   }
-  hipLaunchKernelGGL((lora_small<F16>), dim3((unsigned)z.slots, (unsigned)z.Rp / 4, 2), dim3(256), 0, stream, sp[0], sp[1]);
-  expand<F16>(e, stream);
-  GradParams g{};
-  g.rows = rows; g.R = p.R; g.Rp = (int)z.Rp; g.P = (int)z.P; g.chunk = (int)z.chunk; g.slots = (int)z.slots;
-  g.vec_store = p.R % 4 == 0 && p.K % 4 == 0 && (uintptr_t)p.grad_a % 8 == 0 && (uintptr_t)p.grad_b % 8 == 0;
-  for (int j = 0; j < 2; ++j) {
-    GradJob& job = g.job[j];
-    job.big = (const uint16_t*)(j ? p.x : p.y);
-    job.ld = j ? p.ldx : p.ldy;
-    job.hi = b.hi[j]; job.lo = b.lo[j]; job.up = b.up[j];
-    job.grad = (uint16_t*)(j ? p.grad_a : p.grad_b);
-    job.part = b.sums[j];
-    job.C = j ? p.K : p.N;
-    job.vec = job.C % 8 == 0 && job.ld % 8 == 0 && aligned16(job.big);
-    job.blocks = (job.C + 255) / 256;
-  }
-  switch (rank_blocks(p.R)) {
-    case 1: launch_grad<F16, 1>(g, stream); break;
-    case 2: launch_grad<F16, 2>(g, stream); break;
-    case 4: launch_grad<F16, 4>(g, stream); break;
-    default: launch_grad<F16, 8>(g, stream); break;
-  }
-  const int blocks0 = (int)(((int64_t)p.N * p.R + 1023) / 1024), blocks1 = (int)(((int64_t)p.K * p.R + 1023) / 1024);
-  hipLaunchKernelGGL((lora_grad_sum<F16>), dim3(blocks0 + blocks1, p.L), dim3(256), 0, stream, g, blocks0);
+  expand<F16, true>(e, stream);
+  const int blocks0 = (int)(((int64_t)p.N * p.R + 2047) / 2048), blocks1 = (int)(((int64_t)p.K * p.R + 2047) / 2048);
+  hipLaunchKernelGGL((lora_grad_sum<F16>), dim3(blocks0 + blocks1, p.L), dim3(256), 0, stream, g[0], g[1], blocks0);
 }
 
 }  // namespace
 
 size_t lora_forward_workspace(int64_t T, int L, int K, int N, int R) {
+  if (one_kernel(T, K, R)) return 0;
   const Sizes z = sizes_of(T, L, K, N, R);
   return (size_t)z.s_x * z.P * z.Rp * sizeof(float);
 }
 
 size_t lora_backward_workspace(int64_t T, int L, int K, int N, int R, bool with_h) {
   Workspace w{nullptr, 0};
-  backward_space(w, sizes_of(T, L, K, N, R), L, K, N, R, with_h);
+  backward_space(w, sizes_of(T, L, K, N, R), T, K, N, R, with_h);
   return w.used;
 }
 

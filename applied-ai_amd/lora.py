@@ -103,11 +103,11 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     lib = _lib.lib()
     nbytes = lib.moe_gg_lora_add_workspace(T, L, K, N, R)
     with _ops._on_device(dev):
-        workspace = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=dev)
+        workspace = x.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
         rc = lib.moe_gg_lora_add(y.data_ptr(), _ld(y), x.data_ptr(), _ld(x), a.data_ptr(), b.data_ptr(), None if scales is None else scales.data_ptr(),
                                  plan.perm.data_ptr(), plan.offsets.data_ptr(), L, T, K, N, R, out.data_ptr(), _ld(out),
-                                 h.data_ptr() if return_h else None, 1 if x.dtype == torch.float16 else 0, workspace.data_ptr(),
-                                 workspace.numel(), _ops._stream_ptr(dev))
+                                 h.data_ptr() if return_h else None, 1 if x.dtype == torch.float16 else 0, workspace.data_ptr() if nbytes else None,
+                                 nbytes, _ops._stream_ptr(dev))
     if rc:
         _lib.check(rc, "moe_gg_lora_add")
     return (out, h) if return_h else out

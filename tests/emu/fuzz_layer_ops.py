@@ -60,12 +60,12 @@ def c_lora(rng):
     dt = H.FP16 if fp16 else H.BF16
     out, h = H._full((T, N), H.NAN16, np.uint16), H._full((T, R), np.nan, np.float32)
     nb = L.moe_gg_lora_add_workspace(T, n, K, N, R)
-    H.ok(L.moe_gg_lora_add(P(y), N, P(x), K, P(a), P(b), P(s), P(perm), P(off), n, T, K, N, R, P(out), N, P(h), dt, work(nb), max(nb, 256), None))
+    H.ok(L.moe_gg_lora_add(P(y), N, P(x), K, P(a), P(b), P(s), P(perm), P(off), n, T, K, N, R, P(out), N, P(h), dt, work(nb), nb, None))
     gx, ga, gb = H._full((T, K), H.NAN16, np.uint16), H._full((n, R, K), H.NAN16, np.uint16), H._full((n, N, R), H.NAN16, np.uint16)
     keep = rng.random() < 0.5
     nb = L.moe_gg_lora_backward_workspace(T, n, K, N, R, int(keep))
     H.ok(L.moe_gg_lora_backward(P(g), N, P(x), K, P(a), P(b), P(s), P(perm), P(off), n, T, K, N, R, P(h) if keep else None, P(gi), K, P(gx), K, P(ga), P(gb), dt,
-                                work(nb), max(nb, 256), None))
+                                work(nb), nb, None))
     if corrupt:
         return
     hw, ow, gxw, gaw, gbw = np.zeros((T, R)), yf.copy(), gif.copy(), np.zeros((n, R, K)), np.zeros((n, N, R))
@@ -119,7 +119,7 @@ def c_norm(rng):
     ggate = out((d,), wide_w) if kind == 1 else out((T,), wide_w) if kind == 2 else None
     nb = L.moe_gg_block_norm_backward_workspace(T, d)
     H.ok(L.moe_gg_block_norm_backward(P(gh), d, P(gz) if pre else None, d, P(y), d, P(h), d, P(wp), P(gt), kind, P(wn), 0.9, 0.5, 1e-6, P(gy), P(gr), P(gpost), P(ggate),
-                                      P(gpre), T, d, dt, ds, dw, work(nb), max(nb, 256), None))
+                                      P(gpre), T, d, dt, ds, dw, work(nb), nb, None))
     hs = h.astype(np.float64) if wide else H.from16(h, fp16).astype(np.float64)
     tot = ghf.copy()
     if pre:

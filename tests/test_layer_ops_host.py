@@ -63,10 +63,10 @@ def test_c_abi_refusals_of_the_norms(lib):
 
 
 def test_c_abi_refusals_of_the_adapters(lib):
-    ws = lib.moe_gg_lora_add_workspace(6, 2, 16, 24, 4)
-    assert ws > 0 and lib.moe_gg_lora_add_workspace(6, 2, 16, 24, 129) == 0
+    ws = lib.moe_gg_lora_add_workspace(600, 2, 16, 24, 4)
+    assert ws > 0 and lib.moe_gg_lora_add_workspace(600, 2, 16, 24, 129) == 0 and lib.moe_gg_lora_add_workspace(6, 2, 16, 24, 4) == 0
 
-    def add(y=P, ldy=24, x=P, ldx=16, a=P, b=P, scales=None, perm=P, offsets=P, L=2, T=6, K=16, N=24, R=4, out=P, ldo=24, h=None, dtype=0, work=P, nbytes=ws):
+    def add(y=P, ldy=24, x=P, ldx=16, a=P, b=P, scales=None, perm=P, offsets=P, L=2, T=600, K=16, N=24, R=4, out=P, ldo=24, h=None, dtype=0, work=P, nbytes=ws):
         return lib.moe_gg_lora_add(y, ldy, x, ldx, a, b, scales, perm, offsets, L, T, K, N, R, out, ldo, h, dtype, work, nbytes, None)
     for absent in ("y", "x", "a", "b", "perm", "offsets", "out", "work"):
         assert add(**{absent: None}) == EINVAL, absent
@@ -76,10 +76,10 @@ def test_c_abi_refusals_of_the_adapters(lib):
         assert add(**big) == EUNSUPPORTED
     assert add(x=P + 1) == EALIGN and add(work=P + 8) == EALIGN and add(scales=P + 2) == EALIGN
     assert add(T=0, y=None) == 0
-    wb = lib.moe_gg_lora_backward_workspace(6, 2, 16, 24, 4, 0)
+    wb = lib.moe_gg_lora_backward_workspace(600, 2, 16, 24, 4, 0)
 
     def back(go=P, ldg=24, x=P, ldx=16, perm=P, offsets=P, h=None, gin=None, ld_in=16, gx=P, ld_gx=16, ga=P, gb=P, work=P, nbytes=wb):
-        return lib.moe_gg_lora_backward(go, ldg, x, ldx, P, P, None, perm, offsets, 2, 6, 16, 24, 4, h, gin, ld_in, gx, ld_gx, ga, gb, 0, work, nbytes, None)
+        return lib.moe_gg_lora_backward(go, ldg, x, ldx, P, P, None, perm, offsets, 2, 600, 16, 24, 4, h, gin, ld_in, gx, ld_gx, ga, gb, 0, work, nbytes, None)
     for absent in ("go", "x", "perm", "offsets", "gx", "ga", "gb", "work"):
         assert back(**{absent: None}) == EINVAL, absent
     assert back(ldg=23) == ESHAPE and back(gin=P, ld_in=15) == ESHAPE and back(gin=P, ld_in=24) == ESHAPE and back(nbytes=wb - 1) == EINVAL

@@ -51,12 +51,12 @@ struct Slot {
   int padded;  // the same row's place among the 16-padded intermediates
   int begin;   // position of the group's first row
   int size;    // rows of the group
+  int of;      // the group that owns the slot, also where it holds nothing
 };
 
-DEVINL bool slots_are_rows(const Rows& r, int unit) { return r.T < r.T / unit + r.G; }
-DEVINL Slot slot_of(const Rows& r, int v, int unit, int g, int begin, int end) {
+DEVINL Slot slot_of(bool by_row, int v, int unit, int g, int begin, int end) {
   int skip = (v - (begin / unit + g)) * unit;
-  if (slots_are_rows(r, unit)) skip = (v - begin) % unit == 0 ? v - begin : -1;
+  if (by_row) skip = (v - begin) % unit == 0 ? v - begin : -1;
   Slot s;
   s.begin = begin;
   s.size = end - begin;
@@ -64,17 +64,17 @@ DEVINL Slot slot_of(const Rows& r, int v, int unit, int g, int begin, int end) {
   s.rows = min(unit, s.size - skip);
   s.padded = 16 * (begin / 16 + g) + skip;
   s.group = s.rows > 0 && skip >= 0 ? g : -1;
+  s.of = g;
   return s;
 }
 // Which rows slot v of `unit` rows holds. All lanes of the wave take part; the result is the same in all of them. Whatever
 // the table holds, the rows named lie inside [0, T).
-DEVINL Slot find_slot(const Rows& r, int v, int unit) {
+DEVINL Slot find_slot(const Rows& r, int v, int unit, bool by_row) {
   const int lane = lane_id();
-  const bool by_row = slots_are_rows(r, unit);
   if (r.G < 64) {  // the whole table in one load
     const int off = clamp_off(r, min(lane, r.G));
     const int g = min(max(__popcll(__ballot(lane < r.G && (by_row ? off : off / unit + lane) <= v)) - 1, 0), r.G - 1);
-    return slot_of(r, v, unit, g, __shfl(off, g, 64), __shfl(off, g + 1, 64));
+    return slot_of(by_row, v, unit, g, __shfl(off, g, 64), __shfl(off, g + 1, 64));
   }
   const int step = (r.G + 63) >> 6;
   int i = lane * step;
@@ -88,8 +88,9 @@ DEVINL Slot find_slot(const Rows& r, int v, int unit) {
     g += max(__popcll(__ballot(le)) - 1, 0);
   }
   g = min(g, r.G - 1);
-  return slot_of(r, v, unit, g, clamp_off(r, g), clamp_off(r, g + 1));
+  return slot_of(by_row, v, unit, g, clamp_off(r, g), clamp_off(r, g + 1));
 }
+DEVINL Slot find_slot(const Rows& r, int v, int unit) { return find_slot(r, v, unit, r.T < r.T / unit + r.G); }
 
 // Eight elements at any address: the hardware's wide loads and stores need no alignment, and what an unaligned one costs
 // is the second line that it may touch.
@@ -539,82 +540,41 @@ __global__ __launch_bounds__(1024) void lora_few(ShrinkParams f, ExpandParams p,
   if (mine && !(none && p.out == p.y)) strip.finish(p, none, t, c0, hs, row_up);
 }
 
-// ---- backward: the [rows, R] operand of wgrad ---------------------------------------------------------------------------
-// From the splits' parts (or from h as the forward pass returned it, in row order): for rank r and padded row n
-// hi[r][n], lo[r][n] = the two 16-bit parts of s_g * value, for fp16 times the power of two that suits the largest of 32 rows
-// (one step of wgrad); up[padded row / 16][r] is its inverse, for the first of the 32 rows. sum (may be null) is the sum of the parts for expand.
-struct SmallParams {
-  const float* part;
-  const float* h;  // instead of part, [T, R]
-  const float* scales;
-  Rows rows;
-  int R, Rp, P, splits;
-  uint16_t* hi;  // [Rp][P]
-  uint16_t* lo;
-  float* up;     // [P / 16][Rp]
-  float* sum;    // [P][Rp]
-};
-
-// A workgroup takes 32 rows. A thread takes four ranks of one of them; the 32 threads of a rank are neighbours. The parts are
-// dealt to as many strands of threads as there are threads for, whose sums meet in LDS.
-template <bool F16>
-__global__ __launch_bounds__(1024) void lora_small(SmallParams p) {
+// ---- backward: the sum of many parts ------------------------------------------------------------------------------------
+// out[row][r] = the parts' sum. A workgroup takes 32 rows, a thread four ranks of one of them; the parts are dealt to as many
+// strands of threads as there are threads for, whose sums meet in LDS.
+__global__ __launch_bounds__(1024) void lora_sum(const float* parts, int splits, Rows rows, int Rp, int P, float* out) {
   __shared__ f32x4_t strands[1024];
-  const Slot s = find_slot(p.rows, blockIdx.x, 32);
-  if (s.group < 0 || s.group == p.rows.G - 1) return;
-  const int n = threadIdx.x & 31, quads = p.Rp / 4, quad = (threadIdx.x >> 5) % quads, strand = (threadIdx.x >> 5) / quads;
-  const int many = 32 / quads, r = 4 * quad;  // Rp <= 128: at least one strand
-  const float scale = p.scales ? p.scales[s.group] : 1.f;
+  const Slot s = find_slot(rows, blockIdx.x, 32);
+  if (s.group < 0 || s.group == rows.G - 1) return;
+  const int n = threadIdx.x & 31, quads = Rp / 4, quad = (threadIdx.x >> 5) % quads, strand = (threadIdx.x >> 5) / quads;
+  const int many = 32 / quads;  // Rp <= 128: at least one strand
+  const int64_t next = (int64_t)P * Rp, at = (int64_t)(s.padded + n) * Rp + 4 * quad;
   f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-  if (p.h) {
-    const int t = strand == 0 && n < s.rows ? p.rows.perm[s.first + n] : -1;
-    if (t >= 0 && t < p.rows.T)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (r + e < p.R) v[e] = p.h[(int64_t)t * p.R + r + e];
-  } else if (strand < many && n < s.rows) {
-    const int64_t next = (int64_t)p.P * p.Rp;
-    v = sum_parts<8>(p.part + (int64_t)(s.padded + n) * p.Rp + r + strand * next, p.splits - strand, many, next);
-  }
+  if (strand < many && n < s.rows) v = sum_parts<8>(parts + at + strand * next, splits - strand, many, next);
   strands[threadIdx.x] = v;
   __syncthreads();
-  if (strand > 0) return;
+  if (strand > 0 || n >= s.rows) return;
   for (int i = 1; i < many; ++i) v += strands[threadIdx.x + 32 * quads * i];
-  if (p.sum && n < s.rows) *(f32x4_t*)(p.sum + (int64_t)(s.padded + n) * p.Rp + r) = v;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float a = v[e] * scale;
-    if (F16) {
-      float m = finite_max(0.f, a);
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) m = max(m, __shfl_xor(m, d, 64));
-      a *= pow2_down(m);
-      if (n == 0) p.up[(int64_t)(s.padded / 16) * p.Rp + r + e] = pow2_up(m);
-    }
-    if (n < ((s.rows + 15) & ~15)) {
-      uint16_t hi, lo;
-      split16<F16>(a, hi, lo);
-      p.hi[(int64_t)(r + e) * p.P + s.padded + n] = hi;
-      p.lo[(int64_t)(r + e) * p.P + s.padded + n] = lo;
-    }
-  }
+  *(f32x4_t*)(out + at) = v;
 }
 
 // ---- backward: wgrad ----------------------------------------------------------------------------------------------------
-// grad[c, r] = sum over the rows of an adapter of big[row, c] * small[row, r]. A workgroup takes up to `chunk` rows, 256
+// grad[c, r] = sum over the rows of an adapter of big[row, c] * s_g small[row, r]. A workgroup takes up to `chunk` rows, 256
 // columns (64 to a wave) and up to 64 ranks, in steps of 32 rows: the rows go through LDS as they are and are read back
-// transposed, the small operand is laid out for the matrix instruction already.
-// An adapter of one chunk is finished here; the sums of several are added in their order by lora_grad_sum, which also clears
-// the gradients of adapters without rows.
-// OUT: big is the output's gradient, grad is gB as [C, R], and the same rows give the columns' share of u = gout B, part u[block]:
-// wave w multiplies rows 16 (w % 2) .. of a step with columns 128 (w / 2) .., whose B it keeps in registers as operands, and
-// the two halves of the columns meet in LDS one step later. Not OUT: big is x, grad is gA as [R, C].
+// transposed; the small operand is split into its two parts on the way into LDS, where it lies as the matrix instruction wants it.
+// fp16: four ranks of a step share a power of two that suits their largest value; a step's products are summed apart and
+// scaled back. An adapter of one chunk is finished here, one without rows is cleared; the sums of several chunks are added in
+// their order by lora_grad_sum.
+// OUT: big is the output's gradient, small h, grad is gB as [C, R], and the same rows give the columns' share of u = gout B,
+// part u[block]: wave w multiplies rows 16 (w % 2) .. of a step with columns 128 (w / 2) .., whose B it keeps in registers
+// as operands, and the two halves of the columns meet in LDS one step later. Not OUT: big is x, small u, grad is gA as [R, C].
 struct GradParams {
   const uint16_t* big;
   int64_t ld;
-  const uint16_t* hi;
-  const uint16_t* lo;
-  const float* up;
+  const float* small;  // by_row: [T, pitch] in row order, else `parts` of [P, pitch]
+  int pitch, parts, by_row;
+  const float* scales;
   uint16_t* grad;      // [L, C, R] or [L, R, C]
   float* part;         // [entries][C * R]
   const uint16_t* b;   // OUT: [L, C, R]
@@ -630,17 +590,28 @@ constexpr int GRAD_TILE = 32 * GRAD_ROW + 4 * GRAD_SKEW;
 
 template <bool F16, int RF, bool OUT>
 __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
-  constexpr int SMALL = 2 * RF * 16 * 4;        // 16-byte pieces of the small operand per step
-  constexpr int SL = (SMALL + 255) / 256;
+  constexpr int SL = (RF * 128 + 255) / 256;  // four ranks of one of 32 rows: RF * 128 of them in a step
   __shared__ __align__(16) uint16_t tile[2][GRAD_TILE];
-  __shared__ __align__(16) uint16_t small[2][SMALL * 8];
+  __shared__ __align__(16) uint16_t small[2][2][RF * 16][32];
+  __shared__ float small_up[2][RF * 4];
   __shared__ f32x4_t half_u[OUT ? 2 : 1][OUT ? 2 * RF : 1][64];
   const int slot = blockIdx.x % p.slots, block = blockIdx.x / p.slots % p.blocks, r0 = blockIdx.x / p.slots / p.blocks * 16 * RF;
-  const Slot s = find_slot(p.rows, slot, p.chunk);
-  if (s.group < 0 || s.group == p.rows.G - 1) return;
+  const Slot s = find_slot(p.rows, slot, p.chunk, false);
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), i16 = lane & 15, q = lane >> 4;
   const int c0 = block * 256, rows16 = (s.rows + 15) & ~15;
+  const int64_t block_size = (int64_t)p.C * p.R;
+  if (s.of == p.rows.G - 1) return;
+  uint16_t* grad = p.grad + s.of * block_size;
+  if (s.group < 0) {
+    if (s.size <= 0 && r0 == 0)  // the one slot of an adapter without rows
+      for (int64_t n = tid; n < (int64_t)min(256, p.C - c0) * p.R; n += 256) {
+        const int64_t c = OUT ? 0 : n % min(256, p.C - c0), r = OUT ? 0 : n / min(256, p.C - c0);
+        grad[OUT ? (int64_t)c0 * p.R + n : r * p.C + c0 + c] = 0;
+      }
+    return;
+  }
   const int cl = c0 + 8 * (tid & 31), some = p.C - cl;  // this thread's eight columns of the rows tid / 32 + 8 j
+  const float scale = p.scales ? p.scales[s.group] : 1.f;
 
   // B of this wave's 128 columns, ranks r0 ..: through the tile, one half of the columns after the other
   u32x4_t bt[OUT ? 4 : 1][RF];
@@ -675,16 +646,19 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int f = 0; f < RF; ++f) acc[j][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  auto row_of = [&](int n, int (&t)[4]) {
+  // rows of the step at n: t[0..3] of the big operand, t[4] of the small one (row tid % 32)
+  auto row_of = [&](int n, int (&t)[5]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      t[j] = n + (tid >> 5) + 8 * j < s.rows ? p.rows.perm[s.first + n + (tid >> 5) + 8 * j] : -1;
+    for (int j = 0; j < 5; ++j) {
+      const int m = n + (j < 4 ? (tid >> 5) + 8 * j : (tid & 31));
+      t[j] = m < s.rows ? p.rows.perm[s.first + m] : -1;
       if (t[j] >= p.rows.T) t[j] = -1;
     }
   };
-  u32x4_t bv[4], sv[SL];
+  u32x4_t bv[4];
+  f32x4_t sv[SL];
   const bool edge = c0 + 256 > p.C;
-  auto load = [&](int n0, const int (&t)[4]) {
+  auto load = [&](int n0, const int (&t)[5]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       bv[j] = u32x4_t{0u, 0u, 0u, 0u};
@@ -694,9 +668,38 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
     }
 #pragma unroll
     for (int j = 0; j < SL; ++j) {
-      const int i = tid + 256 * j, n = n0 + 8 * (i & 3), r = r0 + (i >> 2) % (RF * 16);
-      sv[j] = u32x4_t{0u, 0u, 0u, 0u};
-      if (i < SMALL && n < rows16 && r < p.Rp) sv[j] = load16((i >= SMALL / 2 ? p.lo : p.hi) + (int64_t)r * p.P + s.padded + n);
+      const int i = tid + 256 * j, n = n0 + (i & 31), r = r0 + 4 * (i >> 5);
+      sv[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (i >= RF * 128 || t[4] < 0 || r >= p.R) continue;
+      const float* src = p.small + (int64_t)(p.by_row ? t[4] : s.padded + n) * p.pitch + r;
+      if (r + 4 > p.pitch) {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (r + e < p.pitch) sv[j][e] = src[e];
+      } else {
+        sv[j] = *(const f32x4_any_t*)src;
+        if (p.parts > 1) sv[j] = sum_parts<8>(src, p.parts, 1, (int64_t)p.P * p.pitch);
+      }
+    }
+  };
+  auto put_small = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < SL; ++j) {
+      const int i = tid + 256 * j, n = i & 31, r = 4 * (i >> 5);
+      if (i >= RF * 128) continue;
+      f32x4_t v = sv[j];
+      float f = 1.f;
+      if (F16) {
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = finite_max(m, v[e] * scale);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) m = max(m, __shfl_xor(m, d, 64));
+        f = pow2_down(m);
+        if (n == 0) small_up[buf][r >> 2] = pow2_up(m);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split16<F16>(v[e] * scale * f, small[buf][0][r + e][n], small[buf][1][r + e][n]);
     }
   };
   // this wave's share of u for the rows of the step before, waves 0 and 1: with the other half's
@@ -713,19 +716,17 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
       }
     }
   };
-  int t[4];
+  int t[5];
   row_of(0, t);
   load(0, t);
   row_of(32, t);
   int buf = 0;
   for (int n0 = 0; n0 < s.rows; n0 += 32, buf ^= 1) {
     uint16_t* tl = tile[buf];
-    uint16_t* sm = small[buf];
 #pragma unroll
     for (int j = 0; j < 4; ++j) *(u32x4_t*)(tl + grad_off((tid >> 5) + 8 * j) + 8 * (tid & 31)) = bv[j];
-#pragma unroll
-    for (int j = 0; j < SL; ++j)
-      if (tid + 256 * j < SMALL) *(u32x4_t*)(sm + (tid + 256 * j) * 8) = sv[j];
+    wave_whole();
+    put_small(buf);
     if (n0 + 32 < s.rows) {
       load(n0 + 32, t);
       row_of(n0 + 64, t);
@@ -753,21 +754,15 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
     for (int f = 0; f < RF; ++f) {
       u32x4_t v[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) v[h] = *(const u32x4_t*)(sm + ((h * RF * 16 + 16 * f + i16) * 4 + q) * 8);
+      for (int h = 0; h < 2; ++h) v[h] = *(const u32x4_t*)&small[buf][h][16 * f + i16][8 * q];
       if (F16) {
-        // a step has its own scale for each rank: its products are summed apart and scaled back
-        const int r = r0 + 16 * f + (OUT ? 4 * q : i16);
-        const float* up = p.up + (int64_t)((s.padded + n0) / 16) * p.Rp;
-        f32x4_t scale;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) scale[e] = r + (OUT ? e : 0) < p.Rp ? up[r + (OUT ? e : 0)] : 0.f;
+        const float up = small_up[buf][4 * f + (OUT ? q : i16 >> 2)];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           f32x4_t d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int h = 0; h < 2; ++h) d = OUT ? mfma_16x16x32<F16>(v[h], b[j], d) : mfma_16x16x32<F16>(b[j], v[h], d);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][f][e] += d[e] * scale[e];
+          acc[j][f] += d * up;
         }
       } else {
 #pragma unroll
@@ -782,9 +777,7 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
     write_u((s.rows - 1) & ~31);
   }
   const bool whole = s.size <= p.chunk;
-  const int64_t block_size = (int64_t)p.C * p.R;
   const int64_t entry = s.begin / (p.chunk / 2) + (s.first - s.begin) / p.chunk;
-  uint16_t* grad = p.grad + s.group * block_size;
   float* part = p.part + entry * block_size;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -809,7 +802,7 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
     }
 }
 
-// The gradients of adapters of several chunks, of both jobs; a thread takes eight elements.
+// The gradients of adapters of several chunks, of both products; a thread takes eight elements.
 template <bool F16>
 __global__ __launch_bounds__(256) void lora_grad_sum(GradParams p0, GradParams p1, int blocks0) {
   const int g = blockIdx.y;
@@ -817,12 +810,12 @@ __global__ __launch_bounds__(256) void lora_grad_sum(GradParams p0, GradParams p
   const Rows rows = p0.rows;
   const int chunk = first ? p0.chunk : p1.chunk, C = first ? p0.C : p1.C;
   const int begin = clamp_off(rows, g), size = clamp_off(rows, g + 1) - begin;
-  if (size > 0 && size <= chunk) return;
+  if (size <= chunk) return;
   const int64_t block_size = (int64_t)C * p0.R;
   const int64_t i = ((int64_t)(blockIdx.x - (first ? 0 : blocks0)) * 256 + threadIdx.x) * 8;
   if (i >= block_size) return;
   const int n = (int)min((int64_t)8, block_size - i);
-  const int chunks = size > 0 ? (size + chunk - 1) / chunk : 0;
+  const int chunks = (size + chunk - 1) / chunk;
   const float* part = (first ? p0.part : p1.part) + (int64_t)(begin / (chunk / 2)) * block_size + i;
   uint16_t* d = (first ? p0.grad : p1.grad) + g * block_size + i;
   if (n == 8) {
@@ -901,9 +894,11 @@ int splits_of(int C, int per_wave) { return (C + 8 * per_wave - 1) / (8 * per_wa
 // Few rows, and an A that sixteen waves read in a few microseconds.
 bool one_kernel(int64_t T, int K, int R) { return T <= 128 && R <= 32 && (int64_t)K * rank_blocks(R) <= 8192; }
 
-// Rows of a workgroup of wgrad: 512, or half or a quarter of that until there are about 400 workgroups; with more rows than
-// 8192 more, so that the partial sums of an adapter of several chunks stay at 32 times its gradients.
+// Rows of a workgroup of wgrad: 512, or half or a quarter of that until there are about 400 workgroups, but 512 where that is all
+// there is, which saves the kernel that adds the chunks; with more rows than 8192 more, so that the partial sums of an adapter
+// of several chunks stay at 32 times its gradients.
 int grad_chunk(int64_t T, int C) {
+  if (T <= 512) return 512;
   if (T > 8192) return (int)(512 * ((T + 8191) / 8192));
   int chunk = 512;
   while (chunk > 128 && T / chunk * ((C + 255) / 256) < 384) chunk /= 2;
@@ -939,20 +934,17 @@ struct Workspace {
   }
 };
 
+// With few column blocks the readers of u add its parts themselves.
+bool sum_first(const Sizes& z) { return z.blocks > 8; }
+
 struct BackwardSpace {
-  uint16_t *hi[2], *lo[2];                               // 0: h, 1: u
-  float *part_u, *part_h, *sum_u, *up[2], *sums[2];
+  float *part_u, *part_h, *sum_u, *sums[2];
 };
 BackwardSpace backward_space(Workspace& w, const Sizes& z, int64_t T, int K, int N, int R, bool with_h) {
   BackwardSpace b;
   b.part_u = w.take<float>(z.blocks * z.P * z.Rp);
   b.part_h = with_h ? nullptr : w.take<float>(z.s_x * z.P * z.Rp);
-  b.sum_u = w.take<float>(z.P * z.Rp);
-  for (int j = 0; j < 2; ++j) {
-    b.hi[j] = w.take<uint16_t>(z.Rp * z.P);
-    b.lo[j] = w.take<uint16_t>(z.Rp * z.P);
-    b.up[j] = w.take<float>(z.P / 16 * z.Rp);
-  }
+  b.sum_u = sum_first(z) ? w.take<float>(z.P * z.Rp) : b.part_u;
   b.sums[0] = w.take<float>(grad_entries(T, z.chunk[0]) * N * R);
   b.sums[1] = w.take<float>(grad_entries(T, z.chunk[1]) * K * R);
   return b;
@@ -1013,23 +1005,25 @@ void backward(const LoraParams& p, hipStream_t stream) {
   e.out = (uint16_t*)p.gx; e.ldo = p.ld_gx; e.rows = rows; e.C = p.K; e.R = p.R; e.Rp = (int)z.Rp; e.P = (int)z.P; e.splits = 1;
   if (p.L == 0) return expand<F16, true>(e, stream);
   if (!p.h) shrink<F16>(shrink_params(p, rows, z, b.part_h), stream);
+  e.splits = sum_first(z) ? 1 : (int)z.blocks;
   GradParams g[2] = {};
   for (int j = 0; j < 2; ++j) {  // 0: gB and u from the output's gradient and h; 1: gA from x and u
-    SmallParams sp{};
-    sp.part = j ? b.part_u : b.part_h; sp.h = j ? nullptr : (const float*)p.h; sp.scales = p.scales; sp.rows = rows;
-    sp.R = p.R; sp.Rp = (int)z.Rp; sp.P = (int)z.P; sp.splits = j ? (int)z.blocks : z.s_x;
-    sp.hi = b.hi[j]; sp.lo = b.lo[j]; sp.up = b.up[j]; sp.sum = j ? b.sum_u : nullptr;
-    hipLaunchKernelGGL((lora_small<F16>), dim3(slots_of(p.T, z.G, 32)), dim3(1024), 0, stream, sp);
     g[j].big = (const uint16_t*)(j ? p.x : p.y); g[j].ld = j ? p.ldx : p.ldy;
-    g[j].hi = b.hi[j]; g[j].lo = b.lo[j]; g[j].up = b.up[j];
-    g[j].grad = (uint16_t*)(j ? p.grad_a : p.grad_b); g[j].part = b.sums[j]; g[j].b = (const uint16_t*)p.b; g[j].u = b.part_u;
+    g[j].small = j ? b.sum_u : p.h ? (const float*)p.h : b.part_h;
+    g[j].by_row = !j && p.h; g[j].pitch = g[j].by_row ? p.R : (int)z.Rp; g[j].parts = j ? e.splits : p.h ? 1 : z.s_x;
+    g[j].scales = p.scales; g[j].grad = (uint16_t*)(j ? p.grad_a : p.grad_b); g[j].part = b.sums[j]; g[j].b = (const uint16_t*)p.b; g[j].u = b.part_u;
     g[j].rows = rows; g[j].C = j ? p.K : p.N; g[j].R = p.R; g[j].Rp = (int)z.Rp; g[j].P = (int)z.P;
-    g[j].chunk = z.chunk[j]; g[j].slots = slots_of(p.T, z.G, z.chunk[j]); g[j].blocks = (g[j].C + 255) / 256;
-    j ? launch_grad<F16, false>(g[j], stream) : launch_grad<F16, true>(g[j], stream);
+    g[j].chunk = z.chunk[j]; g[j].slots = (int)(p.T / z.chunk[j] + z.G); g[j].blocks = (g[j].C + 255) / 256;
   }
+  launch_grad<F16, true>(g[0], stream);
+  if (sum_first(z))
+    hipLaunchKernelGGL(lora_sum, dim3(slots_of(p.T, z.G, 32)), dim3(1024), 0, stream, (const float*)b.part_u, (int)z.blocks, rows, (int)z.Rp, (int)z.P, b.sum_u);
+  launch_grad<F16, false>(g[1], stream);
   expand<F16, true>(e, stream);
-  const int blocks0 = (int)(((int64_t)p.N * p.R + 2047) / 2048), blocks1 = (int)(((int64_t)p.K * p.R + 2047) / 2048);
-  hipLaunchKernelGGL((lora_grad_sum<F16>), dim3(blocks0 + blocks1, p.L), dim3(256), 0, stream, g[0], g[1], blocks0);
+  if (p.T > z.chunk[0] || p.T > z.chunk[1]) {  // adapters of several chunks are possible
+    const int blocks0 = (int)(((int64_t)p.N * p.R + 2047) / 2048), blocks1 = (int)(((int64_t)p.K * p.R + 2047) / 2048);
+    hipLaunchKernelGGL((lora_grad_sum<F16>), dim3(blocks0 + blocks1, p.L), dim3(256), 0, stream, g[0], g[1], blocks0);
+  }
 }
 
 }  // namespace

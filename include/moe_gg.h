@@ -321,12 +321,11 @@ int moe_gg_route_gate_backward(const float* grad_weights, const void* logits, in
  * y null: h is not written and z is the norm of the residual as it is (residual_scale must be 1).
  *   y, z device [T, d] bf16 or fp16 (dtype); residual, h device [T, d] in that type or fp32 (stream_dtype);
  *   w_post, w_pre device [d], gate device [d] (gate_kind = MOE_GG_GATE_CHANNEL) or [T] (MOE_GG_GATE_ROW), all in dtype or
- *   fp32 (weight_dtype); ldy, ldr: elements between rows; h and z are contiguous. h may be the residual's memory, z y's.
+ *   fp32 (weight_dtype); ldy, ldr: elements between rows; h and z are contiguous and overlap no input.
  * fp32 arithmetic, one rounding per output. d <= MOE_GG_MAX_NORM_WIDTH, T <= 2^21.
  * Backward: h the stored sum (the residual where y is null), grad_h (null: zeros) and grad_z the gradients of both outputs;
  * grad_y [T, d], grad_residual [T, d], grad_w_post, grad_w_pre, grad_gate like their tensors. Outputs that belong to an absent
- * input are null. No two of the outputs and no output and input share memory, but grad_residual may be grad_h's and
- * grad_y grad_z's. workspace: moe_gg_block_norm_backward_workspace bytes, 256-byte aligned. Sums over rows are taken
+ * input are null. No two of the outputs and no output and input share memory. workspace: moe_gg_block_norm_backward_workspace bytes, 256-byte aligned. Sums over rows are taken
  * in a fixed order.
  */
 #define MOE_GG_MAX_NORM_WIDTH 16384

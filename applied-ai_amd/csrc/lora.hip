@@ -820,9 +820,15 @@ __global__ __launch_bounds__(256) void lora_grad_sum(GradParams p0, GradParams p
   uint16_t* d = (first ? p0.grad : p1.grad) + g * block_size + i;
   if (n == 8) {
     f32x4_t v[2] = {};
-    for (int c = 0; c < chunks; ++c, part += block_size) {
-      v[0] += *(const f32x4_any_t*)part;
-      v[1] += *(const f32x4_any_t*)(part + 4);
+    for (int c = 0; c < chunks; c += 4) {  // four chunks' loads under way together
+      f32x4_t a[4][2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) a[k][b] = *(const f32x4_any_t*)(part + min(c + k, chunks - 1) * block_size + 4 * b);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c + k < chunks) v[0] += a[k][0], v[1] += a[k][1];
     }
     store16(d, u32x4_t{pack_16x2<F16>(v[0][0], v[0][1]), pack_16x2<F16>(v[0][2], v[0][3]), pack_16x2<F16>(v[1][0], v[1][1]), pack_16x2<F16>(v[1][2], v[1][3])});
     return;

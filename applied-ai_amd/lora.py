@@ -70,21 +70,13 @@ def _check(rows: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor
     return _ops._require_cuda(rows, x, a, b, perm, offsets, scales), L, T, K, N, R
 
 
-def _row_major(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy, with neighbouring elements of a row next to each other and rows that do not overlap."""
-    return t if t.is_contiguous() or (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
-
-
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _result(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch.Tensor:
+def _result(out: Optional[torch.Tensor], like: torch.Tensor, name: str):
+    """(out or a new tensor like `like`, its elements from row to row)."""
     if out is None:
-        return torch.empty_like(like, memory_format=torch.contiguous_format)
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or _row_major(out) is not out:
+        return _ops._empty_like(like), like.shape[1]
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or _ops._row_major(out)[0] is not out:
         raise ValueError(f"{name} must be a row-major tensor of shape {tuple(like.shape)} and {like.dtype} on the inputs' device")
-    return out
+    return out, _ops._row_major(out)[1]
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: LoraPlan, scales: Optional[torch.Tensor] = None,
@@ -95,17 +87,16 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     out may be y itself. return_h=True returns (out, h) with h = a[e] @ x[t] in fp32 [T, R] (zeros without an adapter), which
     lora_backward takes. fp32 accumulation, one rounding of the result."""
     dev, L, T, K, N, R = _check(y, x, a, b, plan, scales, "y")
-    x, inplace = _row_major(x), out is y
-    if not inplace:
-        y = _row_major(y)
-    out = _result(out, y, "out")
+    x, ldx = _ops._row_major(x)
+    out, ldo = _result(out, y, "out")
+    y, ldy = _ops._row_major(y)  # (y itself where out is y: out is row-major)
     h = x.new_empty((T, R), dtype=torch.float32) if return_h else None
     lib = _lib.lib()
     nbytes = lib.moe_gg_lora_add_workspace(T, L, K, N, R)
     with _ops._on_device(dev):
         workspace = x.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
-        rc = lib.moe_gg_lora_add(y.data_ptr(), _ld(y), x.data_ptr(), _ld(x), a.data_ptr(), b.data_ptr(), None if scales is None else scales.data_ptr(),
-                                 plan.perm.data_ptr(), plan.offsets.data_ptr(), L, T, K, N, R, out.data_ptr(), _ld(out),
+        rc = lib.moe_gg_lora_add(y.data_ptr(), ldy, x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), None if scales is None else scales.data_ptr(),
+                                 plan.perm.data_ptr(), plan.offsets.data_ptr(), L, T, K, N, R, out.data_ptr(), ldo,
                                  h.data_ptr() if return_h else None, 1 if x.dtype == torch.float16 else 0, workspace.data_ptr() if nbytes else None,
                                  nbytes, _ops._stream_ptr(dev))
     if rc:
@@ -128,19 +119,18 @@ def lora_backward(grad_out: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: t
         raise ValueError(f"grad_x must be a {x.dtype} tensor of shape {tuple(x.shape)} on the inputs' device")
     if T == 0:
         h = None
-    x, grad_out = _row_major(x), _row_major(grad_out)
-    if grad_x is not None and out is not grad_x:
-        grad_x = _row_major(grad_x)
-    out = _result(out, x, "out")
+    out, ldo = _result(out, x, "out")
+    (x, ldx), (grad_out, ldg) = _ops._row_major(x), _ops._row_major(grad_out)
+    grad_x, ld_in = (None, 0) if grad_x is None else _ops._row_major(grad_x)
     grad_a, grad_b = torch.empty_like(a), torch.empty_like(b)
     lib = _lib.lib()
     nbytes = lib.moe_gg_lora_backward_workspace(T, L, K, N, R, 0 if h is None else 1)
     with _ops._on_device(dev):
-        workspace = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=dev)
-        rc = lib.moe_gg_lora_backward(grad_out.data_ptr(), _ld(grad_out), x.data_ptr(), _ld(x), a.data_ptr(), b.data_ptr(),
+        workspace = x.new_empty((max(nbytes, 256),), dtype=torch.uint8)
+        rc = lib.moe_gg_lora_backward(grad_out.data_ptr(), ldg, x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(),
                                       None if scales is None else scales.data_ptr(), plan.perm.data_ptr(), plan.offsets.data_ptr(), L, T, K, N, R,
                                       None if h is None else h.data_ptr(), None if grad_x is None else grad_x.data_ptr(),
-                                      0 if grad_x is None else _ld(grad_x), out.data_ptr(), _ld(out), grad_a.data_ptr(), grad_b.data_ptr(),
+                                      ld_in, out.data_ptr(), ldo, grad_a.data_ptr(), grad_b.data_ptr(),
                                       1 if x.dtype == torch.float16 else 0, workspace.data_ptr(), workspace.numel(), _ops._stream_ptr(dev))
     if rc:
         _lib.check(rc, "moe_gg_lora_backward")

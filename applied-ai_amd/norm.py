@@ -18,47 +18,44 @@ _NONE, _CHANNEL, _ROW = 0, 1, 2                                    # MOE_GG_GATE
 _TYPES = (torch.bfloat16, torch.float16)
 
 
-def _row_major(t: torch.Tensor) -> torch.Tensor:
-    return t if t.is_contiguous() or (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
-
-
-def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
 def _check(y, stream, post_weight, gate, pre_weight, extra=()):
-    """(device, gate kind, weights' type) of a call on y (or None) and the residual stream, both [T, d]."""
+    """(device, T, d, gate kind, weights' type) of a call on y (or None) and the residual stream, both [T, d]."""
     if stream.dim() != 2:
         raise ValueError("the residual stream must be [T, d]")
-    T, d = stream.shape
+    T, d = shape = stream.shape
     tensors = [stream]
     if y is not None:
-        if y.shape != stream.shape or y.dtype not in _TYPES:
+        dtype = y.dtype
+        if y.shape != shape or dtype not in _TYPES:
             raise ValueError("the block's output must be bf16 or fp16 of the residual stream's shape")
-        if stream.dtype not in (y.dtype, torch.float32):
+        if stream.dtype != dtype and stream.dtype != torch.float32:
             raise ValueError("the residual stream must have the block output's type or be fp32")
         tensors.append(y)
-    kind = _NONE
+    kind, wt = _NONE, None
     if gate is not None:
         kind = _CHANNEL if gate.shape == (d,) else _ROW if gate.shape == (T, 1) else -1
         if kind < 0:
             raise ValueError(f"the gate must be [{d}] (per channel) or [{T}, 1] (per row)")
-    wt = None
-    for t in (post_weight, gate, pre_weight):
-        if t is None:
-            continue
-        if t is not gate and t.shape != (d,):
-            raise ValueError(f"a norm's weight must be [{d}]")
-        wt = wt or t.dtype
-        if t.dtype != wt or not t.is_contiguous():
-            raise ValueError("the norms' weights and the gate must be contiguous and of one type")
-        tensors.append(t)
-    tensors += [t for t in extra if t is not None]
-    return _ops._require_cuda(*tensors), kind, wt
+        wt = gate.dtype
+        tensors.append(gate)
+        if not gate.is_contiguous():
+            raise ValueError("the gate must be contiguous")
+    for t in (post_weight, pre_weight):
+        if t is not None:
+            if t.shape != (d,) or not t.is_contiguous():
+                raise ValueError(f"a norm's weight must be contiguous [{d}]")
+            if wt is not None and t.dtype != wt:
+                raise ValueError("the norms' weights and the gate must be of one type")
+            wt = t.dtype
+            tensors.append(t)
+    for t in extra:
+        if t is not None:
+            tensors.append(t)
+    return _ops._require_cuda(*tensors), T, d, kind, wt
 
 
 def block_norm(y: torch.Tensor, residual: torch.Tensor, post_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
@@ -71,17 +68,17 @@ def block_norm(y: torch.Tensor, residual: torch.Tensor, post_weight: Optional[to
 
     rms(v) = v / sqrt(mean(v^2) + eps). y bf16 or fp16; residual and h in y's type or fp32; gate [d] or [T, 1]; weights and gate
     in y's type or fp32, all alike; z in y's type. z is computed from h before its rounding. d <= 16384."""
-    dev, kind, wt = _check(y, residual, post_weight, gate, pre_weight)
-    if wt is not None and wt not in (y.dtype, torch.float32):
+    dev, T, d, kind, wt = _check(y, residual, post_weight, gate, pre_weight)
+    dtype = y.dtype
+    if wt is not None and wt != dtype and wt != torch.float32:
         raise ValueError("weights and gate must have the block output's type or be fp32")
-    y, residual = _row_major(y), _row_major(residual)
-    T, d = y.shape
-    h = torch.empty_like(residual, memory_format=torch.contiguous_format)
-    z = torch.empty_like(y, memory_format=torch.contiguous_format) if pre_weight is not None else None
+    (y, ldy), (residual, ldr) = _ops._row_major(y), _ops._row_major(residual)
+    h = _ops._empty_like(residual)
+    z = _ops._empty_like(y) if pre_weight is not None else None
     with _ops._on_device(dev):
-        rc = _lib.lib().moe_gg_block_norm(y.data_ptr(), _ld(y), residual.data_ptr(), _ld(residual), _ptr(post_weight), _ptr(gate), kind, _ptr(pre_weight),
-                                          residual_scale, block_scale, eps, h.data_ptr(), _ptr(z), T, d, _DTYPE[y.dtype], _DTYPE[residual.dtype],
-                                          _DTYPE[wt or y.dtype], _ops._stream_ptr(dev))
+        rc = _lib.lib().moe_gg_block_norm(y.data_ptr(), ldy, residual.data_ptr(), ldr, _ptr(post_weight), _ptr(gate), kind, _ptr(pre_weight),
+                                          residual_scale, block_scale, eps, h.data_ptr(), _ptr(z), T, d, _DTYPE[dtype], _DTYPE[residual.dtype],
+                                          _DTYPE[wt or dtype], _ops._stream_ptr(dev))
     if rc:
         _lib.check(rc, "moe_gg_block_norm")
     return h, z
@@ -97,11 +94,11 @@ def block_norm_backward(grad_h: Optional[torch.Tensor], grad_z: Optional[torch.T
 
 
 def _backward(grad_h, grad_z, y, h, post_weight, gate, pre_weight, residual_scale, block_scale, eps):
-    dev, kind, wt = _check(y, h, post_weight, gate, pre_weight, (grad_h, grad_z))
+    dev, T, d, kind, wt = _check(y, h, post_weight, gate, pre_weight, (grad_h, grad_z))
     if (pre_weight is None) != (grad_z is None):
         raise ValueError("grad_z goes with pre_weight: give both or neither")
     dtype = y.dtype if y is not None else grad_z.dtype
-    if dtype not in (torch.bfloat16, torch.float16) or h.dtype not in (dtype, torch.float32):
+    if dtype not in _TYPES or h.dtype not in (dtype, torch.float32):
         raise ValueError("rows must be bf16 or fp16, the residual stream in that type or fp32")
     if wt is not None and wt not in (dtype, torch.float32):
         raise ValueError("weights and gate must have the block output's type or be fp32")
@@ -109,17 +106,15 @@ def _backward(grad_h, grad_z, y, h, post_weight, gate, pre_weight, residual_scal
         raise ValueError(f"grad_z must be {dtype} {tuple(h.shape)}")
     if grad_h is not None and (grad_h.shape != h.shape or grad_h.dtype != h.dtype):
         raise ValueError(f"grad_h must be {h.dtype} {tuple(h.shape)}")
-    T, d = h.shape
-    y, h, grad_h, grad_z = (None if t is None else _row_major(t) for t in (y, h, grad_h, grad_z))
-    grad_y = None if y is None else torch.empty_like(y, memory_format=torch.contiguous_format)
-    grad_residual = torch.empty_like(h, memory_format=torch.contiguous_format)
+    (y, ldy), (h, ldh), (grad_h, ldgh), (grad_z, ldgz) = ((None, 0) if t is None else _ops._row_major(t) for t in (y, h, grad_h, grad_z))
+    grad_y = None if y is None else _ops._empty_like(y)
+    grad_residual = _ops._empty_like(h)
     grad_post, grad_gate, grad_pre = (None if t is None else torch.empty_like(t) for t in (post_weight, gate, pre_weight))
     lib = _lib.lib()
     nbytes = lib.moe_gg_block_norm_backward_workspace(T, d)
     with _ops._on_device(dev):
-        workspace = torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=dev)
-        rc = lib.moe_gg_block_norm_backward(_ptr(grad_h), 0 if grad_h is None else _ld(grad_h), _ptr(grad_z), 0 if grad_z is None else _ld(grad_z),
-                                            _ptr(y), 0 if y is None else _ld(y), h.data_ptr(), _ld(h), _ptr(post_weight), _ptr(gate), kind,
+        workspace = h.new_empty((max(nbytes, 256),), dtype=torch.uint8)
+        rc = lib.moe_gg_block_norm_backward(_ptr(grad_h), ldgh, _ptr(grad_z), ldgz, _ptr(y), ldy, h.data_ptr(), ldh, _ptr(post_weight), _ptr(gate), kind,
                                             _ptr(pre_weight), residual_scale, block_scale, eps, _ptr(grad_y), grad_residual.data_ptr(),
                                             _ptr(grad_post), _ptr(grad_gate), _ptr(grad_pre), T, d, _DTYPE[dtype], _DTYPE[h.dtype],
                                             _DTYPE[wt or dtype], workspace.data_ptr(), workspace.numel(), _ops._stream_ptr(dev))
@@ -132,16 +127,15 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, dtype: Op
     """x / sqrt(mean(x^2) + eps) * weight: the norm in front of a block on its own. x [T, d] bf16, fp16 or fp32; weight [d] in
     the result's type or fp32. The result has x's type, or dtype (bf16 or fp16, needed for fp32 x)."""
     dtype = dtype or x.dtype
-    dev, _, wt = _check(None, x, None, None, weight)
+    dev, T, d, _, wt = _check(None, x, None, None, weight)
     if dtype not in (torch.bfloat16, torch.float16) or x.dtype not in (dtype, torch.float32):
         raise ValueError("the result must be bf16 or fp16, x of that type or fp32")
     if wt not in (dtype, torch.float32):
         raise ValueError("the weight must have the result's type or be fp32")
-    x = _row_major(x)
-    T, d = x.shape
+    x, ldx = _ops._row_major(x)
     z = x.new_empty((T, d), dtype=dtype)
     with _ops._on_device(dev):
-        rc = _lib.lib().moe_gg_block_norm(None, 0, x.data_ptr(), _ld(x), None, None, _NONE, weight.data_ptr(), 1.0, 1.0, eps, None, z.data_ptr(), T, d,
+        rc = _lib.lib().moe_gg_block_norm(None, 0, x.data_ptr(), ldx, None, None, _NONE, weight.data_ptr(), 1.0, 1.0, eps, None, z.data_ptr(), T, d,
                                           _DTYPE[dtype], _DTYPE[x.dtype], _DTYPE[wt], _ops._stream_ptr(dev))
     if rc:
         _lib.check(rc, "moe_gg_block_norm")

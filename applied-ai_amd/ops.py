@@ -28,12 +28,23 @@ def _on_device(device: torch.device):
     return _HERE if device.index is not None and torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def _row_major(t: torch.Tensor):
+    """(t or a copy, elements from row to row) of a matrix: neighbouring elements of a row next to each other, rows apart."""
+    if not t.is_contiguous():
+        if (t.stride(1) == 1 or t.shape[1] == 1) and t.shape[0] > 1 and t.stride(0) >= t.shape[1]:
+            return t, t.stride(0)
+        t = t.contiguous()
+    return t, t.shape[1]
+
+
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _require_cuda(*tensors: torch.Tensor) -> torch.device:
     dev = tensors[0].device
     for t in tensors:
-        if t.is_cuda and t.device == dev:
-            continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise RuntimeError(
                 "applied_ai_amd ops run on a HIP device only (got a %s tensor); there is no CPU path"
                 % t.device.type

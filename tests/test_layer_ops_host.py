@@ -123,3 +123,17 @@ def test_random_calls_against_guard_pages():
     for p in runs:
         log = p.communicate(timeout=900)[0].decode()
         assert p.returncode == 0 and "done 40" in log, log[-2000:]
+
+
+@pytest.mark.skipif(not os.path.exists(build_emu.CXX), reason="host clang++ of the ROCm toolchain not found: the emulated build needs it")
+def test_no_data_race_between_the_waves_of_a_workgroup():
+    """Every kernel of these operators under the race check of tests/emu (each wave a fiber of the thread sanitizer): no two
+    accesses by different waves to the same LDS or global bytes without a barrier between them."""
+    out = os.path.dirname(build_emu.build_race_check())
+    exe = os.path.join(out, "race_layer_ops")
+    objs = [os.path.join(out, f.replace(".hip", ".emu.o")) for f in build_emu.sources()] + [os.path.join(out, f + ".o") for f in ("race_selftest", "emu_core")]
+    subprocess.run([build_emu.CXX, "-fsanitize=thread", "-x", "c++", os.path.join(EMU, "race_layer_ops.cpp"), "-x", "none", "-o", exe] + objs + ["-ldl", "-lpthread"], check=True)
+    for seed in ("0", "5"):
+        p = subprocess.run([exe], env=dict(os.environ, EMU_SEED=seed), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, timeout=900)
+        log = p.stdout.decode()
+        assert p.returncode == 0 and "data race" not in log and "returned an error: 0" in log, log[-3000:]

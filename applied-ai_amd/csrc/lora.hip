@@ -99,11 +99,19 @@ typedef u32x2_t u32x2_any_t __attribute__((aligned(2)));
 typedef f32x4_t f32x4_any_t __attribute__((aligned(4)));
 DEVINL u32x4_t load16(const uint16_t* p) { return *(const u32x4_any_t*)p; }
 DEVINL void store16(uint16_t* p, u32x4_t v) { *(u32x4_any_t*)p = v; }
-// Eight elements p[0..7] of which only the first n exist (none for n <= 0).
-DEVINL u32x4_t load_some(const uint16_t* p, int n) {
+// Eight elements p[0..7] of which only the first n exist (none for n <= 0), with `before` elements in front of p: from the
+// eight that end with the last one where there are as many.
+DEVINL u32x4_t load_some(const uint16_t* p, int n, int before) {
   u32x4_t v = {0u, 0u, 0u, 0u};
+  if (n > 0 && n + before >= 8) {
+    const u32x4_t w = load16(p - (8 - n));
+    const uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
+    const int s = 16 * (8 - n);  // 16 .. 112
+    const uint64_t a = s < 64 ? lo >> (s & 63) | hi << ((64 - s) & 63) : hi >> ((s - 64) & 63), b = s < 64 ? hi >> (s & 63) : 0;
+    return u32x4_t{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)};
+  }
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
+  for (int e = 0; e < 7; ++e)
     if (e < n) v[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
   return v;
 }
@@ -173,9 +181,9 @@ DEVINL void shrink_columns(const uint16_t* const (&xr)[MF], const uint16_t* cons
       const int n = k1 - (k0 + 8 * q + 32 * b);
       u32x4_t xv[MF], wv[NF];
 #pragma unroll
-      for (int i = 0; i < MF; ++i) xv[i] = n >= 8 ? load16(xr[i] + k0 + 32 * b) : load_some(xr[i] + k0 + 32 * b, n);
+      for (int i = 0; i < MF; ++i) xv[i] = n >= 8 ? load16(xr[i] + k0 + 32 * b) : load_some(xr[i] + k0 + 32 * b, n, k0 + 8 * q + 32 * b);
 #pragma unroll
-      for (int j = 0; j < NF; ++j) wv[j] = n >= 8 ? load16(wr[j] + k0 + 32 * b) : load_some(wr[j] + k0 + 32 * b, n);
+      for (int j = 0; j < NF; ++j) wv[j] = n >= 8 ? load16(wr[j] + k0 + 32 * b) : load_some(wr[j] + k0 + 32 * b, n, k0 + 8 * q + 32 * b);
       wave_whole();
 #pragma unroll
       for (int i = 0; i < MF; ++i)
@@ -323,7 +331,7 @@ struct Strip {
         for (int b = 0; b < 2; ++b) {
           const int n = p.C - c - 32 * b;
           if (!EDGE || n >= 8) y[i][b] = load16(src + 32 * b);
-          else y[i][b] = load_some(src + 32 * b, n);
+          else y[i][b] = load_some(src + 32 * b, n, c + 32 * b);
         }
       }
 #pragma unroll
@@ -338,7 +346,7 @@ struct Strip {
         const int r = 8 * k + (lane_id() >> 3), cw = c0 + 8 * (lane_id() & 7), n = r < p.R ? p.C - cw : 0;
         const uint16_t* src = p.w + ((int64_t)group * p.R + r) * p.C + cw;
         if (EDGE ? n >= 8 : r < p.R) w[k >> 2][k & 3] = load16(src);
-        else if (EDGE && n > 0) w[k >> 2][k & 3] = load_some(src, n);
+        else if (EDGE && n > 0) w[k >> 2][k & 3] = load_some(src, n, cw);
       }
     } else {
       const bool whole = p.R % 8 == 0;
@@ -349,7 +357,7 @@ struct Strip {
           const int cw = min(c0 + 32 * (j >> 1) + 8 * (i16 >> 2) + 4 * (j & 1) + (i16 & 3), p.C - 1), r = 16 * k + 8 * (q & 1);
           const uint16_t* src = p.w + ((int64_t)group * p.C + cw) * p.R + r;
           if (whole) w[k][j] = r < p.R ? load16(src) : w[k][j];
-          else w[k][j] = r + 8 <= p.R ? load16(src) : load_some(src, p.R - r);
+          else w[k][j] = r + 8 <= p.R ? load16(src) : load_some(src, p.R - r, cw > 8 ? 8 : cw * p.R + r);
         }
     }
   }
@@ -619,34 +627,6 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
   const int cl = c0 + 8 * (tid & 31), some = p.C - cl;  // this thread's eight columns of the rows tid / 32 + 8 j
   const float scale = p.scales ? p.scales[s.group] : 1.f;
 
-  // B of this wave's 128 columns, ranks r0 ..: through the tile, one half of the columns after the other
-  u32x4_t bt[OUT ? 4 : 1][RF];
-  if (OUT) {
-    constexpr int ROW = RF * 16 + 8;
-    static_assert(128 * ROW <= 2 * GRAD_TILE, "128 columns of B fit the tiles");
-    uint16_t* at = tile[0];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      for (int n = tid; n < 128 * RF * 2; n += 256) {
-        const int c = c0 + 128 * half + n / (RF * 2), r = r0 + 8 * (n % (RF * 2));
-        u32x4_t v = {0u, 0u, 0u, 0u};
-        if (c < p.C) {
-          const uint16_t* src = p.b + ((int64_t)s.group * p.C + c) * p.R + r;
-          if (r + 8 <= p.R) v = load16(src);
-          else if (r < p.R) v = load_some(src, p.R - r);
-        }
-        *(u32x4_t*)(at + (n / (RF * 2)) * ROW + 8 * (n % (RF * 2))) = v;
-      }
-      __syncthreads();
-      if ((wave >> 1) == half)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int f = 0; f < RF; ++f) bt[k][f] = read_transposed(at + (32 * k + 8 * q + (i16 >> 2)) * ROW + 16 * f + 4 * (i16 & 3), 4 * ROW * 2);
-      __syncthreads();
-    }
-  }
-
   f32x4_t acc[4][RF], au[RF];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -670,7 +650,7 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
       bv[j] = u32x4_t{0u, 0u, 0u, 0u};
       const uint16_t* src = p.big + (int64_t)max(t[j], 0) * p.ld + cl;
       if (!edge) bv[j] = t[j] >= 0 ? load16(src) : bv[j];
-      else if (t[j] >= 0) bv[j] = some >= 8 ? load16(src) : load_some(src, some);
+      else if (t[j] >= 0) bv[j] = some >= 8 ? load16(src) : load_some(src, some, cl);
     }
 #pragma unroll
     for (int j = 0; j < SL; ++j) {
@@ -724,8 +704,45 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
   };
   int t[5];
   row_of(0, t);
+  // B of this wave's 128 columns, ranks r0 ..: through the tile, one half of the columns after the other. Its loads and the
+  // first step's are under way together.
+  u32x4_t bt[OUT ? 4 : 1][RF], staged[OUT ? 2 : 1][RF];
+  constexpr int ROW = RF * 16 + 8;
+  static_assert(128 * ROW <= 2 * GRAD_TILE, "128 columns of B fit the tiles");
+  if (OUT)
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int i = 0; i < RF; ++i) {
+        const int n = tid + 256 * i, c = c0 + 128 * half + n / (RF * 2), r = r0 + 8 * (n % (RF * 2));
+        u32x4_t v = {0u, 0u, 0u, 0u};
+        if (c < p.C) {
+          const uint16_t* src = p.b + ((int64_t)s.group * p.C + c) * p.R + r;
+          if (r + 8 <= p.R) v = load16(src);
+          else if (r < p.R) v = load_some(src, p.R - r, c > 8 ? 8 : c * p.R + r);
+        }
+        staged[OUT ? half : 0][i] = v;
+      }
   load(0, t);
   row_of(32, t);
+  if (OUT) {
+    uint16_t* at = tile[0];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int i = 0; i < RF; ++i) {
+        const int n = tid + 256 * i;
+        *(u32x4_t*)(at + (n / (RF * 2)) * ROW + 8 * (n % (RF * 2))) = staged[OUT ? half : 0][i];
+      }
+      __syncthreads();
+      if ((wave >> 1) == half)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int f = 0; f < RF; ++f) bt[OUT ? k : 0][f] = read_transposed(at + (32 * k + 8 * q + (i16 >> 2)) * ROW + 16 * f + 4 * (i16 & 3), 4 * ROW * 2);
+      __syncthreads();
+    }
+  }
   int buf = 0;
   for (int n0 = 0; n0 < s.rows; n0 += 32, buf ^= 1) {
     uint16_t* tl = tile[buf];
@@ -733,20 +750,21 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
     for (int j = 0; j < 4; ++j) *(u32x4_t*)(tl + grad_off((tid >> 5) + 8 * j) + 8 * (tid & 31)) = bv[j];
     wave_whole();
     put_small(buf);
+    __syncthreads();
+    // stores before loads: a wave waits for its memory operations in their order, and the next step waits for these loads
+    if (OUT && n0 > 0) write_u(n0 - 32);
     if (n0 + 32 < s.rows) {
       load(n0 + 32, t);
       row_of(n0 + 64, t);
     }
-    __syncthreads();
     if (OUT) {
-      if (n0 > 0) write_u(n0 - 32);
 #pragma unroll
       for (int f = 0; f < RF; ++f) au[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const u32x4_t v = *(const u32x4_t*)(tl + grad_off(16 * (wave & 1) + i16) + 128 * (wave >> 1) + 32 * k + 8 * q);
 #pragma unroll
-        for (int f = 0; f < RF; ++f) au[f] = mfma_16x16x32<F16>(v, bt[k][f], au[f]);
+        for (int f = 0; f < RF; ++f) au[f] = mfma_16x16x32<F16>(v, bt[OUT ? k : 0][f], au[f]);
       }
       if (wave >= 2)
 #pragma unroll

@@ -135,7 +135,8 @@ template <bool F16> DEVINL void split16(float v, uint16_t& hi, uint16_t& lo) {
 // ---- shrink -------------------------------------------------------------------------------------------------------------
 // part[split][padded row][r] = sum over the split's columns of x[row, c] * w[group, r, c].
 // A workgroup takes MF x 16 rows and one split; its eight waves take an eighth of the split each and are summed through LDS.
-// A row is read by four lanes, 64 consecutive bytes at a time.
+// A row is read by four lanes, 64 consecutive bytes at a time. Bound by the latency of its chain of loads (group table, rows, columns)
+// and by HBM: 4096 x 4096 bf16, rank 16, 14 us (2.4 TB/s); 64 rows of 14336 and 32 adapters 8 us.
 struct ShrinkParams {
   const uint16_t* x;
   int64_t ldx;
@@ -270,6 +271,7 @@ __global__ __launch_bounds__(512) void lora_shrink(ShrinkParams p, int slots) {
 // strip, operand row i of fragment j is column 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4: a lane's results are twice eight
 // consecutive columns of one row, and the four lanes of a row store 64 consecutive bytes.
 // WT: w is [group, r, c] (the backward pass with A): a strip of it goes through the wave's LDS and is read back transposed.
+// Bound by HBM: 4096 rows of 14336 bf16 read and written in 58 us (4.0 TB/s; a copy reaches 4.9); non-temporal stores take 68 us.
 struct ExpandParams {
   const float* part;
   const uint16_t* w;  // [L, C, R], WT: [L, R, C]
@@ -577,6 +579,8 @@ __global__ __launch_bounds__(1024) void lora_sum(const float* parts, int splits,
 // OUT: big is the output's gradient, small h, grad is gB as [C, R], and the same rows give the columns' share of u = gout B,
 // part u[block]: wave w multiplies rows 16 (w % 2) .. of a step with columns 128 (w / 2) .., whose B it keeps in registers
 // as operands, and the two halves of the columns meet in LDS one step later. Not OUT: big is x, small u, grad is gA as [R, C].
+// Bound by the steps' barriers and latency: OUT on 4096 x 14336 bf16, rank 16, 41 us (3.2 TB/s with what it writes of u), x of 4096 x 4096
+// 14 us. Loads two steps ahead (49 us, registers), steps of 64 rows (46 us) and chunks of 256 rows (42 us) were no faster.
 struct GradParams {
   const uint16_t* big;
   int64_t ld;

@@ -300,7 +300,8 @@ int moe_gg_fp8_block128_quant(const void* in, int dtype, void* out, float* scale
  *   p = softmax(logits) over the row, or sigmoid(logits) (score); ids = the k largest logits of the row, descending, ties to
  *   the lower id, NaN below every number; weights[t, j] = scale * p[t, ids[t, j]], with renormalize != 0 divided by the sum
  *   of the chosen p. A row whose chosen logits are all -infinity has weights (and gradients) of zero.
- *   logits device [T, E] (dtype: fp32, bf16 or fp16); weights device out fp32 [T, k]; ids device out int32 [T, k]
+ *   logits device [T, E] (dtype: fp32, bf16 or fp16), finite, -infinity or NaN (which makes NaN of the weights that it enters:
+ *   other rows do not notice); weights device out fp32 [T, k]; ids device out int32 [T, k]
  * Backward: grad_weights device fp32 [T, k], logits and ids as above, grad_logits device out [T, E] in the logits' type. An id
  * outside [0, E) takes no part; an id named twice counts twice.
  * E <= MOE_GG_MAX_ROUTE_EXPERTS, k <= min(E, 64), T <= 2^24. fp32 arithmetic.

@@ -196,3 +196,57 @@ def test_long_tensors_norms():
     (norm(hs) * v).sum().backward()
     assert bool(((gres[rows].double() - hs.grad).abs() <= 2.0 ** -8 * hs.grad.abs() + fp32).all())
     assert bool(gy.isfinite().all()) and bool(gpost.isfinite().all()) and bool(gpre.isfinite().all())
+
+
+def test_storage_that_begins_at_any_element():
+    """Contiguous tensors whose first element lies 2 bytes (fp32: 4) past an aligned address: the same bits as aligned ones."""
+    import applied_ai_amd as A
+
+    def off_by_one(t):
+        raw = torch.zeros(t.numel() + 9, dtype=t.dtype, device=t.device)
+        v = raw[1:1 + t.numel()].view(t.shape)
+        v.copy_(t)
+        return v
+
+    g = torch.Generator().manual_seed(6)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    T, K, N, R, L = 40, 136, 72, 16, 3
+    x, y, a, b, go, gx = (v.to(BF).cuda() for v in (r(T, K), r(T, N), r(L, R, K), r(L, N, R), r(T, N), r(T, K)))
+    s, ids = torch.rand(L, generator=g).cuda(), torch.randint(-1, L, (T,), generator=g, dtype=torch.int32).cuda()
+    plan = A.lora_plan(ids, L)
+    want = A.lora_add(y, x, a, b, plan, s, return_h=True)
+    got = A.lora_add(*(off_by_one(v) for v in (y, x, a, b)), A.LoraPlan(off_by_one(plan.perm), off_by_one(plan.offsets)), off_by_one(s), return_h=True)
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    back = A.lora_backward(go, x, a, b, plan, s, h=want[1], grad_x=gx)
+    got = A.lora_backward(off_by_one(go), off_by_one(x), off_by_one(a), off_by_one(b), plan, s, h=off_by_one(want[1]), grad_x=off_by_one(gx))
+    assert all(torch.equal(p, q) for p, q in zip(back, got))
+    st, w, gate, gh, gz = r(T, K).cuda(), r(K).cuda(), r(K).cuda(), r(T, K).cuda(), r(T, K).to(BF).cuda()
+    want = A.block_norm(x, st, w, gate, w)
+    got = A.block_norm(*(off_by_one(v) for v in (x, st, w, gate, w)))
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    back = A.block_norm_backward(gh, gz, x, want[0], w, gate, w)
+    got = A.block_norm_backward(*(off_by_one(v) for v in (gh, gz, x, want[0], w, gate, w)))
+    assert all(torch.equal(p, q) for p, q in zip(back, got))
+    logits = r(T, 20).to(BF).cuda()
+    weights, chosen = A.route_gate(logits, 3)
+    got = A.route_gate(off_by_one(logits), 3)
+    assert torch.equal(weights, got[0]) and torch.equal(chosen, got[1])
+    assert torch.equal(A.route_gate_backward(weights, logits, chosen), A.route_gate_backward(off_by_one(weights), off_by_one(logits), off_by_one(chosen)))
+
+
+def test_nothing_is_written_beside_the_results():
+    """In-place results in the middle of a larger buffer leave what is around them."""
+    import applied_ai_amd as A
+
+    for T, N in ((5, 33), (600, 264)):
+        g = torch.Generator().manual_seed(T)
+        r = lambda *s: torch.randn(*s, generator=g).to(BF).cuda()  # noqa: E731
+        raw = torch.full(((T + 4) * (N + 5),), 7.0, dtype=BF, device="cuda")
+        wide = raw.view(T + 4, N + 5)
+        y = wide[2:T + 2, 3:N + 3]
+        y.copy_(r(T, N))
+        ids = torch.randint(-1, 2, (T,), generator=g, dtype=torch.int32).cuda()
+        A.lora_add(y, r(T, 48), r(2, 12, 48), r(2, N, 12), A.lora_plan(ids, 2), out=y)
+        around = wide.clone()
+        around[2:T + 2, 3:N + 3] = 7.0
+        assert bool((around == 7.0).all())

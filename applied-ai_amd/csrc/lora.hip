@@ -30,7 +30,6 @@
 
 namespace {
 
-typedef __attribute__((__vector_size__(2 * sizeof(uint16_t)))) uint16_t u16x2_t;
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 
 template <int N> struct Number { static constexpr int value = N; };

@@ -2,7 +2,8 @@
 against an inaccessible page (tests/emu/harness.py), compared with numpy; plans with entries that name no row among them, of
 which nothing is asked but that no access leaves a tensor. Run by tests/test_layer_ops_host.py in child processes.
 
-usage: fuzz_layer_ops.py SEED CASES"""
+usage: fuzz_layer_ops.py SEED CASES [wide]
+wide: the adapters' kernels on tiles of 64 (32) rows first, which only large calls take."""
 import os
 import sys
 
@@ -39,11 +40,13 @@ def size(rng, hi):
     return max(1, v // 8 * 8) if rng.random() < 0.5 else v
 
 
-def c_lora(rng):
+def c_lora(rng, shape=None):
     L, fp16 = H.lib(), bool(rng.integers(2))
     T = int(rng.choice([1, 2, 15, 16, 17, 40, 511, 512, 600, 1030])) if rng.random() < 0.7 else size(rng, 700)
     K, N, R, n = size(rng, 300), size(rng, 300), int(rng.choice([1, 4, 8, 12, 16, 17, 33, 64, 128])), int(rng.choice([0, 1, 2, 5, 63, 64, 70]))
     corrupt = rng.random() < 0.2
+    if shape:
+        (T, K, N, R, n), corrupt = shape, False
     what = ("lora", T, K, N, R, n, fp16, corrupt)
     print(what, flush=True)
     ids = rng.integers(-1, max(n, 1), T).astype(np.int32)
@@ -165,8 +168,11 @@ def c_gate(rng):
     assert np.isfinite(g if dt == 2 else H.from16(g, dt == 1)).all()
 
 
-def main(seed, cases):
+def main(seed, cases, wide=False):
     rng = np.random.default_rng(seed)
+    for shape in ((1090, 4099, 40, 16, 3), (1090, 24, 4100, 20, 2), (1090, 4096, 17, 36, 2), (1090, 2056, 2050, 72, 2)) if wide else ():
+        c_lora(rng, shape)
+        H.release()
     for _ in range(cases):
         (c_lora, c_norm, c_gate)[int(rng.integers(3))](rng)
         H.release()
@@ -174,4 +180,4 @@ def main(seed, cases):
 
 
 if __name__ == "__main__":
-    main(int(sys.argv[1]), int(sys.argv[2]))
+    main(int(sys.argv[1]), int(sys.argv[2]), "wide" in sys.argv[3:])

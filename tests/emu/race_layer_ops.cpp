@@ -72,7 +72,7 @@ int main() {
   lora(40, 136, 300, 24, 2, false, H);     // one kernel, two rank blocks; several steps of the gradients
   lora(300, 96, 270, 33, 2, true, H);      // two kernels
   lora(600, 72, 2100, 16, 3, false, B);    // u summed first, several column blocks
-  lora(700, 1100, 530, 40, 1, true, B);    // 64-row tiles, chunks of one adapter
+  lora(700, 1100, 530, 40, 1, true, B);    // chunks of one adapter
   lora(530, 64, 72, 100, 2, true, B);      // ranks in two rounds
   norms(5, 500, 1, true, true, B, F, B);
   norms(9, 1030, 2, true, true, H, H, F);

@@ -120,6 +120,14 @@ def test_forward_and_backward(shape, dtype):
         near(g, v, t, what + " alone")
 
 
+@pytest.mark.parametrize("shape", [(4200, 1040, 1111, 16, 5, "random"), (4200, 1040, 1111, 27, 5, "runs"), (4200, 1111, 1040, 64, 3, "random"),
+                                   (4200, 1040, 1040, 128, 3, "runs"), (1300, 4100, 4099, 8, 70, "random")], ids=str)
+def test_long_batches(shape):
+    """The kernels' tiles of 64 (ranks beyond 64: 32) rows, which only calls of many rows and columns take."""
+    test_forward_and_backward(shape, BF)
+    test_forward_and_backward(shape, FP)
+
+
 @pytest.mark.parametrize("pad", [1, 8])
 @pytest.mark.parametrize("T", [37, 600])
 def test_rows_apart_in_place_and_without_scales(T, pad):

@@ -118,7 +118,7 @@ def test_gpu_tests_pass_on_the_emulated_kernels():
 def test_random_calls_against_guard_pages():
     """Random calls with every tensor against an inaccessible page and LDS that starts as NaN, plans of nonsense among them."""
     build_emu.build()
-    runs = [subprocess.Popen([sys.executable, os.path.join(EMU, "fuzz_layer_ops.py"), str(10 + i), "40"], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+    runs = [subprocess.Popen([sys.executable, os.path.join(EMU, "fuzz_layer_ops.py"), str(10 + i), "40", "wide"], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
                              env=dict(os.environ, EMU_GUARD=guard, EMU_LDS_POISON="1")) for i, guard in enumerate(("end", "start"))]
     for p in runs:
         log = p.communicate(timeout=900)[0].decode()

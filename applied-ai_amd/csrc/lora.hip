@@ -21,10 +21,14 @@
 // Where that is fewer, slots are the rows themselves, of which every unit-th of a group has work (a few single tokens beside
 // many loaded adapters).
 //
-// The intermediates are fp32. As matrix operands they are split into a high and a low part of the 16-bit type, which keep
-// 16 (bf16) or 22 (fp16) significant bits: one matrix instruction covers 16 ranks, its 32-deep reduction holding
-// [high 16 | low 16] against the same 16 columns of the other operand twice. For fp16 the rows are scaled by a power of two
-// first, so that neither part leaves the type's range.
+// The intermediates are fp32. As matrix operands they are split into parts of the 16-bit type, each the rounding of what the parts
+// before it leave: three of bf16, which hold all 24 bits, or two of fp16, which hold 22 (a result in fp16 has 11). One matrix
+// instruction covers two parts of 16 ranks, its 32-deep reduction holding [first 16 | second 16] against the same 16 columns of
+// the other operand twice; the third part takes another one. Two parts of bf16 would be off by 2^-17, many times the error of the
+// fp32 sums around them. The third costs nothing at rank 16 (4096 rows of 4096 -> 14336: expand 58 us with and without it, the
+// gradients' kernels 44 + 14 us) and 5 to 16 % of a kernel from rank 64 on, where the matrix instructions count (rank 128: expand
+// 318 -> 341 us, the gradients' 203 -> 217 and 45 -> 46 us). For fp16 the rows are scaled by a power of two first, so that
+// neither part leaves the type's range.
 #include "common.h"
 #include "kernels.h"
 
@@ -124,11 +128,17 @@ DEVINL float finite_max(float m, float v) {
 DEVINL uint32_t scale_exponent(float m) { return min(max(__builtin_bit_cast(uint32_t, m) >> 23, 14u), 253u); }
 DEVINL float pow2_down(float m) { return __builtin_bit_cast(float, (267u - scale_exponent(m)) << 23); }
 DEVINL float pow2_up(float m) { return __builtin_bit_cast(float, (scale_exponent(m) - 13u) << 23); }
-// v as high + low part of the 16-bit type; the low part of an infinity or NaN is 0.
-template <bool F16> DEVINL void split16(float v, uint16_t& hi, uint16_t& lo) {
-  hi = cvt_16<F16>(v);
-  const float r = v - f32_of_16<F16>(hi);
-  lo = __builtin_fabsf(r) <= 3.4028234e38f ? cvt_16<F16>(r) : (uint16_t)0;
+template <bool F16> constexpr int PARTS = F16 ? 2 : 3;
+// v as a sum of parts of the 16-bit type; of an infinity or NaN the first one is all.
+template <bool F16> DEVINL void split16(float v, uint16_t (&part)[PARTS<F16>]) {
+  part[0] = cvt_16<F16>(v);
+  float r = v - f32_of_16<F16>(part[0]);
+  if (!(__builtin_fabsf(r) <= 3.4028234e38f)) r = 0.f;
+#pragma unroll
+  for (int i = 1; i < PARTS<F16>; ++i) {
+    part[i] = cvt_16<F16>(r);
+    r -= f32_of_16<F16>(part[i]);
+  }
 }
 
 // ---- shrink -------------------------------------------------------------------------------------------------------------
@@ -266,7 +276,7 @@ __global__ __launch_bounds__(512) void lora_shrink(ShrinkParams p, int slots) {
 
 // ---- expand -------------------------------------------------------------------------------------------------------------
 // out[row, c] = y[row, c] + s_g sum_r h[row, r] w[group, c, r], h the sum of the splits' parts. A workgroup takes MF x 16
-// rows and `cols` columns: h goes to LDS once as [high | low] operands, every wave takes strips of 64 columns. Of a
+// rows and `cols` columns: h goes to LDS once in its parts, every wave takes strips of 64 columns. Of a
 // strip, operand row i of fragment j is column 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4: a lane's results are twice eight
 // consecutive columns of one row, and the four lanes of a row store 64 consecutive bytes.
 // WT: w is [group, r, c] (the backward pass with A): a strip of it goes through the wave's LDS and is read back transposed.
@@ -304,6 +314,12 @@ template <int MF> DEVINL void lane_rows(const Rows& rows, const Slot& s, int (&t
     if (t[i] >= rows.T) t[i] = -1;
   }
 }
+
+// The parts of a workgroup's rows of h, as the matrix instructions take them.
+template <bool F16, int KF, int MF> struct Parts {
+  uint16_t pair[KF][16 * MF][32];                        // first and second part of 16 ranks
+  uint16_t third[F16 ? 1 : KF][F16 ? 1 : 16 * MF][16];
+};
 
 constexpr int WT_ROW = 72;  // elements from rank to rank of a transposed strip in LDS
 
@@ -392,9 +408,16 @@ struct Strip {
       for (int j = 0; j < 4; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < KF; ++k) {
-        const u32x4_t hv = *(const u32x4_t*)&hs[k][16 * i + i16][8 * q];
+        const u32x4_t hv = *(const u32x4_t*)&hs.pair[k][16 * i + i16][8 * q];
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j] = mfma_16x16x32<F16>(w[k][j], hv, acc[j]);
+        if (!F16) {
+          u32x4_t tv = *(const u32x4_t*)&hs.third[F16 ? 0 : k][F16 ? 0 : 16 * i + i16][8 * (q & 1)];
+          if (q >= 2) tv = u32x4_t{0u, 0u, 0u, 0u};
+          wave_whole();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] = mfma_16x16x32<F16>(w[k][j], tv, acc[j]);
+        }
       }
       const float up = row_up[16 * i + i16];
       if (t[i] >= 0) {
@@ -465,24 +488,23 @@ DEVINL void put_h(const ExpandParams& p, const Slot& s, bool none, bool write_h,
       up = scale * pow2_up(m);
     }
     if (r == 0) row_up[row] = up;
-    uint32_t hi[2], lo[2];
+    uint16_t part[4][PARTS<F16>];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      uint16_t h0, l0, h1, l1;
-      split16<F16>(v[2 * e] * f, h0, l0);
-      split16<F16>(v[2 * e + 1] * f, h1, l1);
-      hi[e] = (uint32_t)h0 | ((uint32_t)h1 << 16);
-      lo[e] = (uint32_t)l0 | ((uint32_t)l1 << 16);
-    }
-    uint16_t* d = &hs[r >> 4][row][r & 15];
-    *(u32x2_t*)d = u32x2_t{hi[0], hi[1]};
-    *(u32x2_t*)(d + 16) = u32x2_t{lo[0], lo[1]};
+    for (int e = 0; e < 4; ++e) split16<F16>(v[e] * f, part[e]);
+    auto put = [&](uint16_t* d, int i) {
+      *(u32x2_t*)d = u32x2_t{(uint32_t)part[0][i] | ((uint32_t)part[1][i] << 16), (uint32_t)part[2][i] | ((uint32_t)part[3][i] << 16)};
+    };
+    put(&hs.pair[r >> 4][row][r & 15], 0);
+    put(&hs.pair[r >> 4][row][16 + (r & 15)], 1);
+    if (!F16) put(&hs.third[F16 ? 0 : r >> 4][F16 ? 0 : row][r & 15], PARTS<F16> - 1);
   }
 }
 
+// Rank 16: four waves to a SIMD, for which the compiler has to be asked (with three of them 73 us; transposed, where it would spill
+// two registers, it makes no difference).
 template <bool F16, int KF, int MF, bool WT>
-__global__ __launch_bounds__(256) void lora_expand(ExpandParams p, int slots) {
-  __shared__ __align__(16) uint16_t hs[KF][16 * MF][32];
+__global__ __launch_bounds__(256, KF == 1 && !WT ? 4 : 1) void lora_expand(ExpandParams p, int slots) {
+  __shared__ __align__(16) Parts<F16, KF, MF> hs;
   __shared__ float row_up[16 * MF];
   __shared__ __align__(16) uint16_t tiles[WT ? 4 : 1][WT ? 16 * KF : 1][WT_ROW];
   const int block = blockIdx.x / slots;
@@ -511,7 +533,7 @@ __global__ __launch_bounds__(256) void lora_expand(ExpandParams p, int slots) {
 // is less than a second launch and a round trip through memory as long as A is small (see one_kernel).
 template <bool F16, int NF>
 __global__ __launch_bounds__(1024) void lora_few(ShrinkParams f, ExpandParams p, int slots) {
-  __shared__ __align__(16) uint16_t hs[NF][16][32];
+  __shared__ __align__(16) Parts<F16, NF, 1> hs;
   __shared__ float row_up[16];
   __shared__ __align__(16) float parts[16][16][16 * NF];
   const int block = blockIdx.x / slots;
@@ -571,7 +593,7 @@ __global__ __launch_bounds__(1024) void lora_sum(const float* parts, int splits,
 // ---- backward: wgrad ----------------------------------------------------------------------------------------------------
 // grad[c, r] = sum over the rows of an adapter of big[row, c] * s_g small[row, r]. A workgroup takes up to `chunk` rows, 256
 // columns (64 to a wave) and up to 64 ranks, in steps of 32 rows: the rows go through LDS as they are and are read back
-// transposed; the small operand is split into its two parts on the way into LDS, where it lies as the matrix instruction wants it.
+// transposed; the small operand is split into its parts on the way into LDS, where it lies as the matrix instruction wants it.
 // fp16: four ranks of a step share a power of two that suits their largest value; a step's products are summed apart and
 // scaled back. An adapter of one chunk is finished here, one without rows is cleared; the sums of several chunks are added in
 // their order by lora_grad_sum.
@@ -603,7 +625,7 @@ template <bool F16, int RF, bool OUT>
 __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
   constexpr int SL = (RF * 128 + 255) / 256;  // four ranks of one of 32 rows: RF * 128 of them in a step
   __shared__ __align__(16) uint16_t tile[2][GRAD_TILE];
-  __shared__ __align__(16) uint16_t small[2][2][RF * 16][32];
+  __shared__ __align__(16) uint16_t small[2][PARTS<F16>][RF * 16][32];
   __shared__ float small_up[2][RF * 4];
   __shared__ f32x4_t half_u[OUT ? 2 : 1][OUT ? 2 * RF : 1][64];
   const int slot = blockIdx.x % p.slots, block = blockIdx.x / p.slots % p.blocks, r0 = blockIdx.x / p.slots / p.blocks * 16 * RF;
@@ -688,7 +710,12 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
         if (n == 0) small_up[buf][r >> 2] = pow2_up(m);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) split16<F16>(v[e] * scale * f, small[buf][0][r + e][n], small[buf][1][r + e][n]);
+      for (int e = 0; e < 4; ++e) {
+        uint16_t part[PARTS<F16>];
+        split16<F16>(v[e] * scale * f, part);
+#pragma unroll
+        for (int h = 0; h < PARTS<F16>; ++h) small[buf][h][r + e][n] = part[h];
+      }
     }
   };
   // this wave's share of u for the rows of the step before, waves 0 and 1: with the other half's
@@ -779,21 +806,21 @@ __global__ __launch_bounds__(256) void lora_grad(GradParams p) {
       b[j] = read_transposed(tl + grad_off(8 * q + (i16 >> 2)) + 64 * wave + 16 * j + 4 * (i16 & 3), 4 * GRAD_ROW * 2);
 #pragma unroll
     for (int f = 0; f < RF; ++f) {
-      u32x4_t v[2];
+      u32x4_t v[PARTS<F16>];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) v[h] = *(const u32x4_t*)&small[buf][h][16 * f + i16][8 * q];
+      for (int h = 0; h < PARTS<F16>; ++h) v[h] = *(const u32x4_t*)&small[buf][h][16 * f + i16][8 * q];
       if (F16) {
         const float up = small_up[buf][4 * f + (OUT ? q : i16 >> 2)];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           f32x4_t d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int h = 0; h < 2; ++h) d = OUT ? mfma_16x16x32<F16>(v[h], b[j], d) : mfma_16x16x32<F16>(b[j], v[h], d);
+          for (int h = 0; h < PARTS<F16>; ++h) d = OUT ? mfma_16x16x32<F16>(v[h], b[j], d) : mfma_16x16x32<F16>(b[j], v[h], d);
           acc[j][f] += d * up;
         }
       } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < PARTS<F16>; ++h)
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[j][f] = OUT ? mfma_16x16x32<F16>(v[h], b[j], acc[j][f]) : mfma_16x16x32<F16>(b[j], v[h], acc[j][f]);
       }

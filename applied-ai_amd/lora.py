@@ -79,17 +79,34 @@ def _result(out: Optional[torch.Tensor], like: torch.Tensor, name: str):
     return out, _ops._row_major(out)[1]
 
 
+def _disjoint(out: torch.Tensor, ld: int, others, name: str) -> None:
+    """others: (tensor or None, bytes from its first element to behind its last one), none of which may share memory with out."""
+    lo = out.data_ptr()
+    hi = lo + 2 * ((out.shape[0] - 1) * ld + out.shape[1])
+    for t, n in others:
+        if t is not None:
+            p = t.data_ptr()
+            if p < hi and lo < p + n and _ops._overlap(out, t):
+                raise ValueError(f"{name} shares memory with an input that other rows of it are computed from")
+
+
 def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: LoraPlan, scales: Optional[torch.Tensor] = None,
              out: Optional[torch.Tensor] = None, return_h: bool = False):
     """out[t] = y[t] + scales[e] * b[e] @ (a[e] @ x[t]) with e the row's adapter; rows without one get y[t].
 
     y [T, N], x [T, K] (rows may lie apart), a [L, R, K], b [L, N, R], all bf16 or all fp16, R <= 128; scales fp32 [L] (default 1).
-    out may be y itself. return_h=True returns (out, h) with h = a[e] @ x[t] in fp32 [T, R] (zeros without an adapter), which
-    lora_backward takes. fp32 accumulation, one rounding of the result."""
+    out may be y itself, but must not share memory with another part of y or with another argument. return_h=True returns
+    (out, h) with h = a[e] @ x[t] in fp32 [T, R] (zeros without an adapter), which lora_backward takes. fp32 accumulation, one
+    rounding of the result."""
     dev, L, T, K, N, R = _check(y, x, a, b, plan, scales, "y")
     x, ldx = _ops._row_major(x)
+    given = out
     out, ldo = _result(out, y, "out")
     y, ldy = _ops._row_major(y)  # (y itself where out is y: out is row-major)
+    if given is not None:
+        same = out is y or (ldo == ldy and out.data_ptr() == y.data_ptr())
+        _disjoint(out, ldo, ((None if same else y, 2 * T * ldy), (x, 2 * T * ldx), (a, 2 * L * R * K), (b, 2 * L * N * R), (scales, 4 * L), (plan.perm, 4 * T),
+                             (plan.offsets, 4 * L + 8)), "out")
     h = x.new_empty((T, R), dtype=torch.float32) if return_h else None
     lib = _lib.lib()
     nbytes = lib.moe_gg_lora_add_workspace(T, L, K, N, R)
@@ -110,7 +127,8 @@ def lora_backward(grad_out: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: t
 
     grad_out [T, N] is the gradient of lora_add's result (and of y as it is). h is what the forward pass returned
     (return_h=True); without it a[e] @ x[t] is computed again. grad_x is the shared projection's part of x's gradient, to
-    which the adapters' is added (default: none); out takes the sum and may be grad_x itself. An adapter without rows gets
+    which the adapters' is added (default: none); out takes the sum and may be grad_x itself, but must not share memory with
+    another part of grad_x, a, scales or the plan. An adapter without rows gets
     zeros. Sums over rows are taken in a fixed order."""
     dev, L, T, K, N, R = _check(grad_out, x, a, b, plan, scales, "grad_out")
     if h is not None and (h.shape != (T, R) or h.dtype != torch.float32 or not h.is_contiguous() or h.device != dev):
@@ -119,9 +137,13 @@ def lora_backward(grad_out: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: t
         raise ValueError(f"grad_x must be a {x.dtype} tensor of shape {tuple(x.shape)} on the inputs' device")
     if T == 0:
         h = None
+    given = out
     out, ldo = _result(out, x, "out")
     (x, ldx), (grad_out, ldg) = _ops._row_major(x), _ops._row_major(grad_out)
     grad_x, ld_in = (None, 0) if grad_x is None else _ops._row_major(grad_x)
+    if given is not None:  # (x, grad_out, b and h have been read when out is written)
+        same = grad_x is None or grad_x is out or (ldo == ld_in and out.data_ptr() == grad_x.data_ptr())
+        _disjoint(out, ldo, ((None if same else grad_x, 2 * T * ld_in), (a, 2 * L * R * K), (scales, 4 * L), (plan.perm, 4 * T), (plan.offsets, 4 * L + 8)), "out")
     grad_a, grad_b = torch.empty_like(a), torch.empty_like(b)
     lib = _lib.lib()
     nbytes = lib.moe_gg_lora_backward_workspace(T, L, K, N, R, 0 if h is None else 1)

@@ -37,6 +37,25 @@ def _row_major(t: torch.Tensor):
     return t, t.shape[1]
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors share an element's memory, each contiguous or a matrix as _row_major gives it (rows of one buffer
+    whose columns belong to different tensors lie between each other and do not)."""
+    def rows(t):  # first byte, bytes from row to row, rows, bytes of a row
+        e = t.element_size()
+        n = t.numel() * e
+        return (t.data_ptr(), n, 1, n) if t.is_contiguous() else (t.data_ptr(), t.stride(0) * e, t.shape[0], t.shape[1] * e)
+
+    (p, dp, n, w), (q, dq, m, v) = sorted((rows(a), rows(b)), key=lambda r: -r[2])
+    if w == 0 or v == 0 or p + (n - 1) * dp + w <= q or q + (m - 1) * dq + v <= p:
+        return False
+    if n > 1 and dp == dq and m > 1:
+        at = (q - p) % dp
+        return at < w or at + v > dp
+    # the first row of the one that ends behind a row of the other begins before that one's end
+    firsts = ((q + i * dq, max(0, (q + i * dq - w - p) // dp + 1)) for i in range(m))
+    return any(k < n and p + k * dp < at + v for at, k in firsts)
+
+
 def _empty_like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 

@@ -1,9 +1,12 @@
-"""More of the adapters, norms and the gate without a GPU: their GPU tests of precision on the emulated build of the kernels."""
+"""More of the adapters, norms and the gate without a GPU: the test of shared memory against a count of bytes, and their GPU tests of
+precision and of shared memory on the emulated build of the kernels."""
 import os
+import random
 import subprocess
 import sys
 
 import pytest
+import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 EMU = os.path.join(ROOT, "tests", "emu")
@@ -12,7 +15,37 @@ sys.path.insert(0, EMU)
 import build_emu  # noqa: E402
 
 emulated = pytest.mark.skipif(not os.path.exists(build_emu.CXX), reason="host clang++ of the ROCm toolchain not found: the emulated build needs it")
-FILES = ["tests/test_gpu_lora_parts.py"]
+FILES = ["tests/test_gpu_lora_parts.py", "tests/test_gpu_layer_ops_memory.py"]
+
+
+def test_shared_memory_is_found_byte_by_byte():
+    """_overlap of views of one buffer, as matrices of equal and of different pitches and as flat tensors, against the sets of their bytes."""
+    from applied_ai_amd import ops
+
+    buffer = torch.zeros(700, dtype=torch.uint8)
+    rng, found = random.Random(5), [0, 0]
+
+    def view():
+        size = rng.choice([1, 1, 2, 4])
+        flat = buffer[:len(buffer) // 4 * 4].view({1: torch.uint8, 2: torch.int16, 4: torch.int32}[size])
+        pitch = rng.choice([12, 12, rng.randint(1, 40)])
+        rows, cols = rng.randint(0, 12), rng.randint(0, pitch)
+        if rng.random() < 0.3:
+            rows, cols, pitch = 1, rng.randint(0, 60), 60
+        rows = min(rows, len(flat) // pitch)
+        start = rng.randint(0, len(flat) - pitch * rows)
+        t = flat.as_strided((rows, cols), (pitch, 1), start)
+        held = {start * size + i * pitch * size + j for i in range(rows) for j in range(cols * size)}
+        assert all(0 <= b < 700 for b in held)
+        return t, held
+
+    for _ in range(20000):
+        (a, p), (b, q) = view(), view()
+        if not all(t.is_contiguous() or (t.shape[0] > 1 and t.stride(0) >= t.shape[1]) for t in (a, b)):
+            continue
+        assert ops._overlap(a, b) == bool(p & q), (a.shape, a.stride(), a.data_ptr() - buffer.data_ptr(), b.shape, b.stride(), b.data_ptr() - buffer.data_ptr())
+        found[bool(p & q)] += 1
+    assert min(found) > 1000
 
 
 @emulated

@@ -844,7 +844,14 @@ int moe_gg_block_norm_backward(const void* grad_h, int64_t ldgh, const void* gra
                                void* workspace, size_t workspace_bytes, void* stream) {
   const int rc = check_norm(T, d, gate_kind, dtype, stream_dtype, weight_dtype);
   if (rc != MOE_GG_OK) return rc;
-  if (d == 0) return MOE_GG_OK;
+  if (d == 0) {  // of all results only a row gate's gradient has elements
+    if (T == 0 || gate_kind != MOE_GG_GATE_ROW) return MOE_GG_OK;
+    if (!grad_gate) return MOE_GG_EINVAL;
+    if (!aligned(grad_gate, weight_dtype == MOE_GG_DTYPE_FP32 ? 4 : 2)) return MOE_GG_EALIGN;
+    NormGradParams p{};
+    p.g_gate = grad_gate; p.gate_kind = gate_kind; p.T = (int)T; p.wide_w = weight_dtype == MOE_GG_DTYPE_FP32;
+    return (int)block_norm_backward_launch(p, dtype == MOE_GG_DTYPE_FP16, (hipStream_t)stream);
+  }
   if ((y != nullptr) != (grad_y != nullptr) || (w_pre != nullptr) != (grad_z != nullptr) || !grad_residual || (w_pre && !h)) {
     if (T != 0) return MOE_GG_EINVAL;
   }

@@ -418,6 +418,14 @@ __global__ __launch_bounds__(256) void block_norm_sums(NormGradParams p) {
   }
 }
 
+// Gates of rows without columns have gradients of zero.
+__global__ __launch_bounds__(256) void block_norm_no_columns(void* g_gate, bool wide, int T) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= T) return;
+  if (wide) ((float*)g_gate)[t] = 0.f;
+  else ((uint16_t*)g_gate)[t] = 0;
+}
+
 // Threads to a row and pieces to a thread by width: a wave up to 512 columns (1024 in the forward pass), else as many threads
 // as keep a row in registers.
 template <bool F16, bool WIDE>
@@ -471,6 +479,10 @@ hipError_t block_norm_launch(const NormParams& p, bool fp16, hipStream_t stream)
 }
 
 hipError_t block_norm_backward_launch(NormGradParams p, bool fp16, hipStream_t stream) {
+  if (p.d == 0) {
+    if (p.T > 0 && p.gate_kind == 2) hipLaunchKernelGGL(block_norm_no_columns, dim3((p.T + 255) / 256), dim3(256), 0, stream, p.g_gate, p.wide_w, p.T);
+    return hipGetLastError();
+  }
   const int grid = grad_grid(p.T, p.d);
   p.parts = grad_parts(p.T, p.d);
   if (p.T > 0) {  // else the sums below are zeros

@@ -15,7 +15,7 @@ sys.path.insert(0, EMU)
 import build_emu  # noqa: E402
 
 emulated = pytest.mark.skipif(not os.path.exists(build_emu.CXX), reason="host clang++ of the ROCm toolchain not found: the emulated build needs it")
-FILES = ["tests/test_gpu_lora_parts.py", "tests/test_gpu_layer_ops_memory.py"]
+FILES = ["tests/test_gpu_lora_parts.py", "tests/test_gpu_layer_ops_memory.py", "tests/test_gpu_norm_rows.py"]
 
 
 def test_shared_memory_is_found_byte_by_byte():

@@ -879,7 +879,8 @@ int moe_gg_block_norm_backward(const void* grad_h, int64_t ldgh, const void* gra
 
 int moe_gg_lora_plan(const int32_t* ids, int64_t T, int L, int32_t* perm, int32_t* offsets, int32_t* scratch, void* stream) {
   if (T < 0 || L < 0) return MOE_GG_EINVAL;
-  if (T > INT32_MAX || L > MOE_GG_MAX_LORA_ADAPTERS) return MOE_GG_EUNSUPPORTED;
+  // the kernels count rows in int, in whole workgroups: T near 2^31 would wrap to rows in front of the tensors
+  if (T > (1 << 30) || L > MOE_GG_MAX_LORA_ADAPTERS) return MOE_GG_EUNSUPPORTED;
   if (!offsets || !scratch || (T > 0 && (!ids || !perm))) return MOE_GG_EINVAL;
   if (!aligned(ids, 4) || !aligned(perm, 4) || !aligned(offsets, 4) || !aligned(scratch, 4)) return MOE_GG_EALIGN;
   return (int)lora_plan_launch(ids, (int)T, L, perm, offsets, scratch, (hipStream_t)stream);

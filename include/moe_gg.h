@@ -361,7 +361,7 @@ int moe_gg_block_norm_backward(const void* grad_h, int64_t ldgh, const void* gra
  * fp32 accumulation; h and u are fp32 and reach the matrix instructions as 16-bit parts, three of bf16 (all 24 bits) or two of
  * fp16 (22 bits, from a power of two that suits the largest of a row's, or of 32 rows of four ranks); each output is rounded once. The
  * order of every sum is fixed by the arguments. a and b must be finite.
- * R <= MOE_GG_MAX_LORA_RANK, L <= MOE_GG_MAX_LORA_ADAPTERS, T <= 2^20, K and N <= 2^17. workspace: moe_gg_lora_*_workspace bytes (0 for a few
+ * R <= MOE_GG_MAX_LORA_RANK, L <= MOE_GG_MAX_LORA_ADAPTERS, T <= 2^20 (moe_gg_lora_plan: 2^30), K and N <= 2^17. workspace: moe_gg_lora_*_workspace bytes (0 for a few
  * rows), 256-byte aligned; nothing in it has to survive a call.
  */
 #define MOE_GG_MAX_LORA_RANK 128

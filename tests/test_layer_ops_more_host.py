@@ -15,6 +15,8 @@ sys.path.insert(0, EMU)
 import build_emu  # noqa: E402
 
 emulated = pytest.mark.skipif(not os.path.exists(build_emu.CXX), reason="host clang++ of the ROCm toolchain not found: the emulated build needs it")
+EUNSUPPORTED = -4
+P = 4096  # an address that is never reached
 FILES = ["tests/test_gpu_lora_parts.py", "tests/test_gpu_layer_ops_memory.py", "tests/test_gpu_norm_rows.py"]
 
 
@@ -57,3 +59,8 @@ def test_gpu_tests_pass_on_the_emulated_kernels():
     for f, p in zip(FILES, runs):
         log = p.communicate(timeout=900)[0].decode()
         assert p.returncode == 0, f + log[-3000:]
+
+
+def test_plans_of_more_rows_than_the_kernels_count_are_refused(lib):
+    for T in ((1 << 30) + 1, 2 ** 31 - 100, 2 ** 31 - 1):
+        assert lib.moe_gg_lora_plan(P, T, 2, P, P, P, None) == EUNSUPPORTED

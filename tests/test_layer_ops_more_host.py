@@ -1,5 +1,5 @@
 """More of the adapters, norms and the gate without a GPU: the test of shared memory against a count of bytes, and their GPU tests of
-precision and of shared memory on the emulated build of the kernels."""
+precision, of shared memory and of many rows on the emulated build of the kernels, and the race check of many rows."""
 import os
 import random
 import subprocess
@@ -17,7 +17,8 @@ import build_emu  # noqa: E402
 emulated = pytest.mark.skipif(not os.path.exists(build_emu.CXX), reason="host clang++ of the ROCm toolchain not found: the emulated build needs it")
 EUNSUPPORTED = -4
 P = 4096  # an address that is never reached
-FILES = ["tests/test_gpu_lora_parts.py", "tests/test_gpu_layer_ops_memory.py", "tests/test_gpu_norm_rows.py"]
+FILES = ["tests/test_gpu_lora_parts.py", "tests/test_gpu_layer_ops_memory.py", "tests/test_gpu_norm_rows.py", "tests/test_gpu_lora_rows.py",
+         "tests/test_gpu_gate_choices.py"]
 
 
 def test_shared_memory_is_found_byte_by_byte():
@@ -64,3 +65,16 @@ def test_gpu_tests_pass_on_the_emulated_kernels():
 def test_plans_of_more_rows_than_the_kernels_count_are_refused(lib):
     for T in ((1 << 30) + 1, 2 ** 31 - 100, 2 ** 31 - 1):
         assert lib.moe_gg_lora_plan(P, T, 2, P, P, P, None) == EUNSUPPORTED
+
+
+@emulated
+def test_no_data_race_from_row_to_row():
+    """The norms' gradients over several rows per workgroup under the race check of tests/emu: LDS that two rows use in turn, and the
+    weights kept there."""
+    out = os.path.dirname(build_emu.build_race_check())
+    exe = os.path.join(out, "race_norm_rows")
+    objs = [os.path.join(out, f.replace(".hip", ".emu.o")) for f in build_emu.sources()] + [os.path.join(out, f + ".o") for f in ("race_selftest", "emu_core")]
+    subprocess.run([build_emu.CXX, "-fsanitize=thread", "-x", "c++", os.path.join(EMU, "race_norm_rows.cpp"), "-x", "none", "-o", exe] + objs + ["-ldl", "-lpthread"], check=True)
+    p = subprocess.run([exe], env=dict(os.environ, EMU_SEED="0"), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, timeout=900)
+    log = p.stdout.decode()
+    assert p.returncode == 0 and "data race" not in log and "returned an error: 0" in log, log[-3000:]

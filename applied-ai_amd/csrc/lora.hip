@@ -967,13 +967,16 @@ bool one_kernel(int64_t T, int64_t G, int K, int N, int R) {
 }
 
 // Rows of a workgroup of wgrad: 512, or half or a quarter of that until there are about 400 workgroups, but 512 where that is all
-// there is, which saves the kernel that adds the chunks; with more rows than 8192 more, so that the partial sums of an adapter
-// of several chunks stay at 32 times its gradients.
+// there is, which saves the kernel that adds the chunks. Beyond 8192 rows also twice, four times .. as many while more than 768
+// workgroups are left, since every chunk of an adapter of several costs a set of partial sums. One adapter, rank 16, all of the
+// backward pass: 65536 rows of 256 columns 150 us with 128 rows to a workgroup and 411 with 4096 (32 workgroups); 16384 of 4096 171
+// with 512 and 207 with 1024; 8192 of 4096 -> 14336, 16 adapters of rank 64, 418 with 512 and 424 with 1024.
 int grad_chunk(int64_t T, int C) {
   if (T <= 512) return 512;
-  if (T > 8192) return (int)(512 * ((T + 8191) / 8192));
+  const int64_t blocks = (C + 255) / 256;
   int chunk = 512;
-  while (chunk > 128 && T / chunk * ((C + 255) / 256) < 384) chunk /= 2;
+  while (chunk > 128 && T / chunk * blocks < 384) chunk /= 2;
+  while (T > 8192 && chunk >= 512 && T / (2 * chunk) * blocks >= 768) chunk *= 2;
   return chunk;
 }
 int64_t grad_entries(int64_t T, int chunk) { return T / (chunk / 2); }

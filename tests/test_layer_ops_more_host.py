@@ -78,3 +78,11 @@ def test_no_data_race_from_row_to_row():
     p = subprocess.run([exe], env=dict(os.environ, EMU_SEED="0"), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, timeout=900)
     log = p.stdout.decode()
     assert p.returncode == 0 and "data race" not in log and "returned an error: 0" in log, log[-3000:]
+
+
+def test_a_longer_batch_keeps_its_partial_sums(lib):
+    """The adapters' gradients of a long batch are cut into as many parts as those of a batch of a row less: fewer leave most of the
+    card without work."""
+    for L, K, N, R in ((1, 256, 256, 16), (1, 1024, 1024, 16), (16, 1024, 1024, 64), (4, 4096, 4096, 16), (2, 300, 14336, 8)):
+        parts = [lib.moe_gg_lora_backward_workspace(T, L, K, N, R, 1) for T in (8191, 8192, 8193, 8200)]
+        assert parts == sorted(parts), (L, K, N, R, parts)

@@ -5,7 +5,8 @@
 //   z = h / sqrt(mean(h^2) + eps) * w_pre       what the next block reads
 // With r = 1 / sqrt(mean(v^2) + eps), the gradient through v * r * w is r * (g w - v r^2 mean(g w v)).
 //
-// Bound by memory: a row is read once into registers, both norms' sums are taken over it there, and everything is written once. Sums are fp32; z is
+// Bound by memory: a row is read once into registers, both norms' sums are taken over it there, and everything is written once (in the
+// backward pass up to 4096 columns; what becomes of wider rows stands there). Sums are fp32; z is
 // computed from the sum before it is rounded to the stream's type. The backward pass starts from the stored stream and
 // computes both norms' r again from the rows, which it reads anyway: nothing but the stream is kept between the passes.
 // Gradients of weights and of a gate per channel are sums over rows: a workgroup adds up its rows in registers, the workgroups'
@@ -197,12 +198,16 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_norm_forward(Norm
 // and gate in LDS (KEEP, where they fit in 64 KB); and the stores behind them are the same in number on every path (FULL: every
 // thread has NV whole pieces of the row), so that the wait for the loads need not wait for them.
 // HAS_Y false: the norm alone.
-// 4096 x 4096 bf16 with a channel gate (201 MB and 25 MB of shares): 41-45 us; without the LDS copies 63, with 512 threads to a row 51,
-// without the row in advance 46.
+// 4096 x 4096 bf16 with a channel gate (201 MB and 25 MB of shares, of which the counters see 92 MB written, as they should): 42 us;
+// without the LDS copies 63, with 512 threads to a row 51, without the row in advance 46.
+// Wider rows are not as fast. Beyond 4096 columns the LDS copies are off (counted at 32 bits they take more than 64 KB) and weights come
+// from memory for every row; two pieces of a row that is not 8192 wide spill 14 to 52 registers, and the 128 registers of
+// each of 1024 threads do not hold two pieces: 134 to 277 go to scratch (without y 10, of an fp32 stream). 4096 rows of 5120 columns 98 us, 7168 121, 8192 115, 12288 369,
+// 16384 613: 2.9 to 3.9 and 1.8 to 1.5 TB/s with the shares.
 template <bool F16, bool WIDE, int TPR, int NV, bool HAS_Y, bool FULL>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR == 1024 ? 4 : 2) void block_norm_backward(NormGradParams p) {
   constexpr int RPB = TPR == 64 ? 4 : 1, STEP = TPR * 8, THREADS = TPR > 256 ? TPR : 256;
-  constexpr bool AHEAD = TPR < 1024;  // the widest rows leave no registers for a second one
+  constexpr bool AHEAD = TPR < 1024;  // the widest rows leave no registers for a second one, nor for all of the first
   constexpr bool KEEP = 3 * NV * THREADS * 32 <= 65536;
   __shared__ float red3[2][TPR / 64][3];
   __shared__ float red2[2][TPR / 64][2];

@@ -281,6 +281,7 @@ __global__ __launch_bounds__(512) void lora_shrink(ShrinkParams p, int slots) {
 // consecutive columns of one row, and the four lanes of a row store 64 consecutive bytes.
 // WT: w is [group, r, c] (the backward pass with A): a strip of it goes through the wave's LDS and is read back transposed.
 // Bound by HBM: 4096 rows of 14336 bf16 read and written in 58 us (4.0 TB/s; a copy reaches 4.9); non-temporal stores take 68 us.
+// Higher ranks hold more of w in registers: 90, 109 and 341 us at rank 32, 64 and 128, with three, two and one waves to a SIMD.
 struct ExpandParams {
   const float* part;
   const uint16_t* w;  // [L, C, R], WT: [L, R, C]
@@ -600,8 +601,9 @@ __global__ __launch_bounds__(1024) void lora_sum(const float* parts, int splits,
 // OUT: big is the output's gradient, small h, grad is gB as [C, R], and the same rows give the columns' share of u = gout B,
 // part u[block]: wave w multiplies rows 16 (w % 2) .. of a step with columns 128 (w / 2) .., whose B it keeps in registers
 // as operands, and the two halves of the columns meet in LDS one step later. Not OUT: big is x, small u, grad is gA as [R, C].
-// Bound by the steps' barriers and latency: OUT on 4096 x 14336 bf16, rank 16, 41 us (3.2 TB/s with what it writes of u), x of 4096 x 4096
-// 14 us. Loads two steps ahead (49 us, registers), steps of 64 rows (46 us) and chunks of 256 rows (42 us) were no faster.
+// Bound by the steps' barriers and latency: OUT on 4096 x 14336 bf16, rank 16, 44 us (3.2 TB/s with what it writes of u), x of 4096 x 4096
+// 14 us. Ranks 32, 64 and 128 take 64, 128 and 216 us for OUT: u's shares grow with the rank, from 64 on one wave to a SIMD is left, and
+// beyond 64 the rows are read once more. Loads two steps ahead (49 us, registers), steps of 64 rows (46 us) and chunks of 256 rows (42 us) were no faster.
 struct GradParams {
   const uint16_t* big;
   int64_t ld;

@@ -200,10 +200,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_norm_forward(Norm
 // HAS_Y false: the norm alone.
 // 4096 x 4096 bf16 with a channel gate (201 MB and 25 MB of shares, of which the counters see 92 MB written, as they should): 42 us;
 // without the LDS copies 63, with 512 threads to a row 51, without the row in advance 46.
-// Wider rows are not as fast. Beyond 4096 columns the LDS copies are off (counted at 32 bits they take more than 64 KB) and weights come
-// from memory for every row; two pieces of a row that is not 8192 wide spill 14 to 52 registers, and the 128 registers of
-// each of 1024 threads do not hold two pieces: 134 to 277 go to scratch (without y 10, of an fp32 stream). 4096 rows of 5120 columns 98 us, 7168 121, 8192 115, 12288 369,
-// 16384 613: 2.9 to 3.9 and 1.8 to 1.5 TB/s with the shares.
+// Wider rows are not as fast. Beyond 4096 columns the LDS copies are off (counted at 32 bits they take more than 64 KB) and weights
+// come from memory for every row; two pieces of a row that is not 8192 wide spill 14 to 52 registers, and the 128 registers of
+// each of 1024 threads do not hold two pieces: 134 to 277 go to scratch (without y 10, of an fp32 stream). 4096 rows of 5120
+// columns 98 us, 7168 121, 8192 115, 12288 369, 16384 613: 2.9 to 3.9 and 1.8 to 1.5 TB/s with the shares.
 template <bool F16, bool WIDE, int TPR, int NV, bool HAS_Y, bool FULL>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256, TPR == 1024 ? 4 : 2) void block_norm_backward(NormGradParams p) {
   constexpr int RPB = TPR == 64 ? 4 : 1, STEP = TPR * 8, THREADS = TPR > 256 ? TPR : 256;

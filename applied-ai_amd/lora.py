@@ -128,8 +128,8 @@ def lora_backward(grad_out: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: t
     grad_out [T, N] is the gradient of lora_add's result (and of y as it is). h is what the forward pass returned
     (return_h=True); without it a[e] @ x[t] is computed again. grad_x is the shared projection's part of x's gradient, to
     which the adapters' is added (default: none); out takes the sum and may be grad_x itself, but must not share memory with
-    another part of grad_x, a, scales or the plan. An adapter without rows gets
-    zeros. Sums over rows are taken in a fixed order."""
+    another part of grad_x, a, scales or the plan. An adapter without rows gets zeros. Sums over rows are taken in a fixed
+    order."""
     dev, L, T, K, N, R = _check(grad_out, x, a, b, plan, scales, "grad_out")
     if h is not None and (h.shape != (T, R) or h.dtype != torch.float32 or not h.is_contiguous() or h.device != dev):
         raise ValueError(f"h must be contiguous fp32 [{T}, {R}] on the inputs' device")
